@@ -22,6 +22,9 @@ from .capi import (  # noqa: F401
     dropout_add_ln_fwd, dropout_add_ln_bwd, dropout_add_ln_bwd_static, dropout_add_ln_fwd_ex, dropout_add_ln_bwd_ex,
     unary, binary_const, binary, broadcast, sce_sparse_bwd_reduced, sce_dense_bwd_reduced, vocab_parallel_ce_gather, vocab_parallel_ce_bwd,
     vocab_parallel_ce_stats, vocab_parallel_ce_combine, vocab_parallel_ce_bwd_fused, UNARY_OPS, BINARY_OPS,
+    token_logprob_fwd, token_logprob_bwd, token_logprob_workspace_bytes, vocab_parallel_logprob_stats,
+    vocab_parallel_logprob_combine, q8_empty, q8_pack, q8_unpack, add_ln_q8_fwd, add_ln_q8_out, add_ln_q8_bwd,
+    add_ln_q8_bwd_workspace_bytes, Q8_BLOCK,
     softmax_fwd, softmax_bwd,
     sce_sparse_fwd, sce_sparse_bwd, sce_dense_fwd, sce_dense_bwd, nll_loss_fwd, nll_loss_bwd,
     reduce, reduce_workspace_bytes, norm, norm_bwd, batch_norm_fwd, batch_norm_bwd, batch_norm_workspace_bytes, tune_set, copy_kernel, strided_copy, strided_scatter, stream_probe, ring_probe, memcpy_d2d,

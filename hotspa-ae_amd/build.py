@@ -24,7 +24,8 @@ INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["hk_norm_bwd_bf16.hip", "hk_norm_bwd_f32.hip", "hk_norm_bwd_f16.hip", "hk_norm_fwd_bf16.hip",
                "hk_norm_fwd_f32.hip", "hk_norm_fwd_f16.hip", "hk_device.hip", "hk_norm.hip", "hk_softmax.hip", "hk_sce.hip", "hk_reduce.hip", "hk_nll.hip",
-               "hk_dropout_ln.hip", "hk_elementwise.hip", "hk_vocab_ce.hip", "hk_batchnorm.hip"]
+               "hk_dropout_ln.hip", "hk_elementwise.hip", "hk_vocab_ce.hip", "hk_batchnorm.hip", "hk_logprob.hip", "hk_q8.hip",
+               "hk_q8_norm_bf16.hip", "hk_q8_norm_f16.hip", "hk_q8_norm_f32.hip"]
 # measurement tools, a library of their own
 BENCH_SOURCES = [os.path.join("bench", "hk_bench_probe.hip")]
 
@@ -57,8 +58,9 @@ def _stale(src, obj):
     if not os.path.exists(obj):
         return True
     own = os.path.getmtime(os.path.join(CSRC, src))
-    # hk_common.h is included by every source; the norm headers only by the norm sources
-    shared = [f for f in os.listdir(CSRC) if f.endswith(".h") and (f == "hk_common.h" or src.startswith("hk_norm"))]
+    # hk_common.h is included by every source; the norm and 8-bit headers only by their sources
+    shared = [f for f in os.listdir(CSRC) if f.endswith(".h") and
+              (f == "hk_common.h" or any(f.startswith(k) and src.startswith(k) for k in ("hk_norm", "hk_q8")))]
     common = max(os.path.getmtime(os.path.join(CSRC, f)) for f in shared)
     header = max(os.path.getmtime(os.path.join(INCLUDE, f)) for f in os.listdir(INCLUDE))
     return os.path.getmtime(obj) < max(own, common, header)

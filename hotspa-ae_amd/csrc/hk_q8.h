@@ -1,0 +1,188 @@
+// Activations kept in 8 bits for the backward pass: rows as blocks of 32 columns that share one power of two (the MXINT8
+// format of the OCP microscaling specification).  Of a block with the largest magnitude a, E = the exponent field of a as
+// fp32 (at least 7), a column holds q = rint(x 2^(133 - E)), cut to [-127, 127], and stands for q 2^(E - 133): off by at
+// most half a step of 2^(E - 133), by less than a whole one past 127.5 steps.  A block with an infinity or a NaN has E = 255
+// and stands for NaN.  The scale is a power of two, so that both directions are exact but for the one rounding to q.
+#pragma once
+
+#include "hk_common.h"
+
+namespace hk {
+
+constexpr int kQ8Block = 32;
+inline int64_t q8_blocks(int64_t cols) { return (cols + kQ8Block - 1) / kQ8Block; }
+
+// A row's columns [c, c + N) of R as floats, c a multiple of N; 0 past the row's end.  TAIL: the row may end inside a
+// vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector inside
+// the row and none sits in a branch.  raw() is the load, floats() what comes of it.
+template <typename R, int N, bool TAIL>
+struct RowVec {
+  static constexpr int M = VecIO<R>::N, K = N / M;   // elements and number of 16-byte loads
+  static_assert(N % M == 0, "whole loads");
+  u32x4 raw[K];
+  // row: any element boundary; one of cols elements, cols >= 1
+  __device__ __forceinline__ void load(const R* row, int c, int cols, bool keep) {
+    if (TAIL && cols < M) {   // uniform: a row shorter than a load
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[k] = u32x4{0, 0, 0, 0};
+      if (c == 0) {
+        float f[M] = {};
+#pragma unroll
+        for (int j = 0; j < M; ++j)
+          if (j < cols) f[j] = Cvt<R>::load(row + j);
+        raw[0] = VecIO<R>::pack(f);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int at = c + k * M, from = min(at, cols - M);
+      raw[k] = keep ? ld16_any_keep<R>(row + from) : ld16_any<R>(row + from);
+    }
+  }
+  __device__ __forceinline__ void floats(float* f, int c, int cols) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      u32x4 r = raw[k];
+      const int at = c + k * M;
+      if constexpr (TAIL) {
+        if (cols >= M) {   // uniform
+          const int bits = (at - min(at, cols - M)) * int(sizeof(R)) * 8;
+          const uint64_t lo = uint64_t(r.y) << 32 | r.x, hi = uint64_t(r.w) << 32 | r.z;
+          const uint64_t in = bits & 63 ? hi << (64 - (bits & 63)) : 0;
+          uint64_t l = bits >= 64 ? hi >> (bits & 63) : (lo >> (bits & 63)) | in, h = bits >= 64 ? 0 : hi >> (bits & 63);
+          if (bits >= 128) l = 0;
+          r = u32x4{uint32_t(l), uint32_t(l >> 32), uint32_t(h), uint32_t(h >> 32)};
+        }
+      } else if (at >= cols) {
+        r = u32x4{0, 0, 0, 0};
+      }
+      VecIO<R>::unpack(r, f + k * M);
+    }
+  }
+};
+
+// stores N floats as R at columns [c, c + N) of a row, those inside it
+template <typename R, int N, bool TAIL>
+__device__ __forceinline__ void store_row_floats(R* row, int c, int cols, const float* f) {
+  constexpr int M = VecIO<R>::N;
+#pragma unroll
+  for (int k = 0; k < N / M; ++k) {
+    const int at = c + k * M, left = cols - at;
+    const u32x4 r = VecIO<R>::pack(f + k * M);
+    if (left >= M) {
+      st16_any(row + at, r);
+    } else if (TAIL && left > 0) {
+      typedef uint32_t word __attribute__((aligned(2)));
+      R* p = row + at;
+      uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      int words = left * int(sizeof(R)) / 4;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < words) reinterpret_cast<word*>(p)[i] = w[i];
+      if (sizeof(R) == 2 && (left & 1)) {
+        const uint32_t last = words == 0 ? w[0] : words == 1 ? w[1] : words == 2 ? w[2] : w[3];
+        reinterpret_cast<uint16_t*>(p)[left - 1] = uint16_t(last);
+      }
+    }
+  }
+}
+
+// The exponent field of the block that this lane's N elements belong to: the 32 / N lanes of a block are neighbours and
+// start at a multiple of their number.  Infinities and NaN have the largest field, 255.
+template <int N>
+__device__ __forceinline__ uint32_t q8_exponent(const float* f) {
+  static_assert(N == 4 || N == 8, "a block is 8 or 4 lanes");
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) m = max(m, f2u(f[j]) & 0x7fffffffu);
+  m = max(m, f2u(dpp_perm<kDppXor1>(u2f(m))));
+  m = max(m, f2u(dpp_perm<kDppXor2>(u2f(m))));
+  if constexpr (N == 4) m = max(m, f2u(dpp_perm<kDppHalfMirror>(u2f(m))));
+  return max(m >> 23, 7u);
+}
+// q of 4 elements in the bytes of a word; factor = 2^(133 - E).  Added to 1.5 * 2^23 a float of that size is rounded to a
+// whole number, ties to even, whose two's complement stands in its lowest bits.
+__device__ __forceinline__ float q8_factor(uint32_t exponent) { return u2f((260u - exponent) << 23); }
+__device__ __forceinline__ uint32_t q8_encode4(const float* f, float factor) {
+  uint32_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = f2u(__builtin_amdgcn_fmed3f(f[j] * factor, -127.f, 127.f) + 12582912.f);
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+  return lo | hi;
+}
+// 2^(E - 133), NaN for E = 255; E below 7 (which q8_exponent never gives) is a subnormal step
+__device__ __forceinline__ float q8_step(uint32_t exponent) {
+  const uint32_t bits = exponent >= 7 ? (exponent - 6) << 23 : 1u << (exponent + 16);
+  return u2f(exponent == 255 ? 0x7fc00000u : bits);
+}
+// the values of 4 bytes
+__device__ __forceinline__ void q8_decode4(uint32_t bytes, float step, float* f) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = float(int8_t(bytes >> (8 * j))) * step;
+}
+
+// the words of N elements, N = 4 or 8
+template <int N> struct Q8Words;
+template <> struct Q8Words<8> {
+  typedef u32x2 type;
+  static __device__ __forceinline__ type encode(const float* f, float factor) {
+    return u32x2{q8_encode4(f, factor), q8_encode4(f + 4, factor)};
+  }
+  static __device__ __forceinline__ void decode(type w, uint32_t exponent, float* f) {
+    const float step = q8_step(exponent);
+    q8_decode4(w.x, step, f);
+    q8_decode4(w.y, step, f + 4);
+  }
+};
+template <> struct Q8Words<4> {
+  typedef uint32_t type;
+  static __device__ __forceinline__ type encode(const float* f, float factor) { return q8_encode4(f, factor); }
+  static __device__ __forceinline__ void decode(type w, uint32_t exponent, float* f) {
+    q8_decode4(w, q8_step(exponent), f);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// what the norm calls are given
+// ---------------------------------------------------------------------------
+struct Q8FwdArgs {
+  const void *x0, *residual, *gamma, *beta;
+  void *z, *x_out;
+  int8_t* q;
+  uint8_t* scale;
+  float *mu, *rs;
+  int64_t x0_pitch, res_pitch, z_pitch, xout_pitch;
+  float eps, inv_cols;
+  int rows, cols, blocks;   // blocks: of 32 columns in a row
+  uint16_t threads;
+};
+struct Q8BwdArgs {
+  const void *dz, *dx_in, *gamma;
+  const int8_t* q;
+  const uint8_t* scale;
+  const float *mu, *rs;
+  void *dx0, *dres;
+  float *part_dgamma, *part_dbeta;
+  int64_t dz_pitch, dxin_pitch, dx_pitch, dres_pitch;
+  float inv_cols;
+  int rows, cols, blocks, grid;
+  uint16_t threads;
+};
+
+constexpr int kQ8MaxCols = 32768;
+
+// Lanes that hold a row and vectors per lane: lanes of a wavefront (8, 16, 32, 64) or, above 64, a workgroup's threads.
+struct Q8Shape {
+  int lanes, nv;
+};
+Q8Shape q8_fwd_shape(int64_t cols, int vec);
+Q8Shape q8_bwd_shape(int64_t cols, int vec);
+// workgroups of the backward kernel
+int q8_bwd_grid(int64_t rows, const Q8Shape& shape);
+
+template <typename T> int q8_norm_fwd_typed(const Q8FwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, hipStream_t s);
+template <typename T> int q8_norm_bwd_typed(const Q8BwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, void* dgamma,
+                                            void* dbeta, hipStream_t s);
+
+} // namespace hk

@@ -140,6 +140,9 @@ template <> struct Arg<float*> : PointerArg<float*> {};
 template <> struct Arg<const float*> : PointerArg<const float*> {};
 template <> struct Arg<uint8_t*> : PointerArg<uint8_t*> {};
 template <> struct Arg<const uint8_t*> : PointerArg<const uint8_t*> {};
+template <> struct Arg<int8_t*> : PointerArg<int8_t*> {};
+template <> struct Arg<const int8_t*> : PointerArg<const int8_t*> {};
+template <> struct Arg<int64_t*> : PointerArg<int64_t*> {};   // written on the device
 // Integers on the host (shape, steps, axes, flags): a tuple, a list or None, never a tensor.
 template <typename I> struct HostArray {
   std::array<I, 16> few;
@@ -355,6 +358,9 @@ PyMethodDef methods[] = {
     ENTRY(hk_sce_dense_bwd_reduced), ENTRY(hk_sce_dense_fwd), LABELS(hk_sce_sparse_bwd_pitched),
     LABELS(hk_sce_sparse_bwd_reduced), LABELS(hk_sce_sparse_fwd_pitched), ENTRY(hk_softmax_bwd),
     ENTRY(hk_softmax_bwd_pitched), ENTRY(hk_softmax_fwd), ENTRY(hk_softmax_fwd_pitched), ENTRY(hk_unary),
+    ENTRY(hk_add_ln_q8_bwd), ENTRY(hk_add_ln_q8_fwd), ENTRY(hk_add_ln_q8_out), ENTRY(hk_q8_pack), ENTRY(hk_q8_unpack),
+    LABELS(hk_token_logprob_bwd), LABELS(hk_token_logprob_fwd), LABELS(hk_vocab_parallel_logprob_combine),
+    LABELS(hk_vocab_parallel_logprob_stats),
 #else
     ENTRY(ht_batch_norm), ENTRY(ht_batch_norm_gradient), ENTRY(ht_binary), ENTRY(ht_binary_const),
     ENTRY(ht_broadcast_shape), ENTRY(ht_dropout_add_ln_bwd), ENTRY(ht_dropout_add_ln_fwd),

@@ -588,6 +588,116 @@ HK_API int hk_vocab_parallel_ce_bwd_fused(int dtype, const void* logits, const i
                                           int64_t ignored_index, hkStream_t stream);
 
 /* ======================================================================== *
+ * Log probabilities of given tokens, with the rows' entropy and their most
+ * likely alternatives, the gradient of the first two, and the same on vocabulary
+ * shards.  What policy training, distillation and scoring take of the logits next
+ * to (or instead of) hk_sce_sparse_*, in one pass over them and in fp32:
+ *   lse[r] = logsumexp(x[r,:]);   logprob[r] = x[r, tokens[r]] - lse[r];
+ *   entropy[r] = -sum_c p log p with p = softmax(x[r,:])        (0 log 0 = 0);
+ *   top_logprob / top_token [rows, top]: the `top` largest logits of the row, minus
+ *   lse, in descending order with their columns; of equal ones the lowest column
+ *   first (0 and -0 are equal).  An element of -inf is no alternative: places that
+ *   are left over hold (-inf, -1).
+ * logits: [rows, cols] fp32 / bf16 / fp16, rows logits_pitch elements apart; tokens:
+ * [rows] int64.  Any of logprob, entropy, lse may be NULL, top may be 0 (at most 32).
+ * A row whose token equals ignored_index is not read and gets 0, 0, 0 and (-inf, -1).
+ * A token outside [0, cols) has a log probability of NaN.  A row that holds a NaN or
+ * +inf, or nothing but -inf, has no distribution: its logprob and entropy are NaN
+ * and so are its alternatives' values, with tokens -1.
+ * Few rows are taken in parts: ask for the workspace (8-byte aligned; may be 0).
+ * No counterpart in the reference, whose loss gives -logprob alone
+ * (hetu/impl/kernel/SoftmaxCrossEntropySparse.cu:239-274).
+ * ======================================================================== */
+HK_API int hk_token_logprob_workspace_bytes(int dtype, int64_t rows, int64_t cols, int64_t top, size_t* bytes);
+HK_API int hk_token_logprob_fwd(int dtype, const void* logits, int64_t logits_pitch, const int64_t* tokens,
+                                float* logprob, float* entropy, float* lse, float* top_logprob,
+                                int64_t* top_token, int64_t top, int64_t rows, int64_t cols,
+                                int64_t ignored_index, void* workspace, size_t workspace_bytes,
+                                hkStream_t stream);
+
+/* With g = grad_logprob[r], h = grad_entropy[r] (fp32, either may be NULL: 0), lse and entropy of the forward
+ * (entropy is read with grad_entropy only):
+ *   dlogits[r, c] = g ([c == tokens[r] - vocab_start] - p_c) - h p_c (log p_c + entropy[r]),  p_c = exp(x[r, c] - lse[r]);
+ * zeros for a row whose token equals ignored_index.  logits are the columns [vocab_start, vocab_start + cols) of
+ * the row: with the merged lse and entropy this is also the gradient of a shard.  dlogits may be logits (the same
+ * address and pitch). */
+HK_API int hk_token_logprob_bwd(int dtype, const void* logits, int64_t logits_pitch, const int64_t* tokens,
+                                const float* lse, const float* entropy, const float* grad_logprob,
+                                const float* grad_entropy, void* dlogits, int64_t dlogits_pitch, int64_t rows,
+                                int64_t cols, int64_t vocab_start, int64_t ignored_index, hkStream_t stream);
+
+/* The same with the vocabulary over several devices; this one holds the columns [vocab_start, vocab_start + cols).
+ *   stats:   in one pass per row of the shard, fp32 [4, rows]: m = the maximum, sum exp(x - m), sum exp(x - m) (x - m),
+ *            and the logit at the token if it lies in the shard, else 0; top_value / top_token [rows, top]: the
+ *            shard's largest logits and their token numbers (vocab_start + column).  (-inf, 0, 0, 0) and (-inf, -1)
+ *            for an ignored row, which is not read.  Workspace as hk_token_logprob_workspace_bytes says.
+ *   combine: stats [nshards, 4, rows] and top_values / top_tokens [nshards, rows, top] as an all-gather leaves them ->
+ *            what hk_token_logprob_fwd gives.  Shards in any order, at most 64.  A token outside [0, vocab_size) has
+ *            a log probability of NaN; vocab_size < 0 leaves that check to negative tokens. */
+HK_API int hk_vocab_parallel_logprob_stats(int dtype, const void* logits, int64_t logits_pitch,
+                                           const int64_t* tokens, float* stats, float* top_value,
+                                           int64_t* top_token, int64_t top, int64_t rows, int64_t cols,
+                                           int64_t vocab_start, int64_t ignored_index, void* workspace,
+                                           size_t workspace_bytes, hkStream_t stream);
+HK_API int hk_vocab_parallel_logprob_combine(const float* stats, const float* top_values,
+                                             const int64_t* top_tokens, int64_t nshards, const int64_t* tokens,
+                                             int64_t ignored_index, int64_t vocab_size, float* logprob,
+                                             float* entropy, float* lse, float* top_logprob, int64_t* top_token,
+                                             int64_t top, int64_t rows, hkStream_t stream);
+
+/* ======================================================================== *
+ * Activations kept in 8 bits for the backward pass, and the norm of a pre-norm
+ * block that keeps its input that way.
+ *
+ * Format (MXINT8 of the OCP microscaling specification): a row is blocks of
+ * HK_Q8_BLOCK = 32 columns, ceil(cols / 32) = nb of them.  scale: [rows, nb] uint8,
+ * E = the exponent field of the block's largest magnitude as fp32, at least 7;
+ * q: [rows, nb * 32] int8, rint(x * 2^(133 - E)) with ties to even, cut to
+ * [-127, 127], 0 behind the row's end.  A column stands for q * 2^(E - 133).  A block
+ * with an infinity or a NaN has E = 255 and stands for NaN.  Both arrays are dense,
+ * q on an 8-byte boundary.  1.03 bytes an element in place of 2 or 4.
+ * x / out: fp32 / bf16 / fp16 rows, a pitch apart.  No counterpart in the reference.
+ * ======================================================================== */
+#define HK_Q8_BLOCK 32
+HK_API int hk_q8_pack(int dtype, const void* x, int64_t x_pitch, int8_t* q, uint8_t* scale, int64_t rows,
+                      int64_t cols, hkStream_t stream);
+HK_API int hk_q8_unpack(int dtype, const int8_t* q, const uint8_t* scale, void* out, int64_t out_pitch,
+                        int64_t rows, int64_t cols, hkStream_t stream);
+
+/* hk_dropout_add_ln_fwd / _bwd (dropout_p = 0) with the pre-norm sum x = x0 + residual (fp32) kept in 8 bits instead
+ * of in rtype, and the norm's output z given back from it, so that a layer keeps 1.03 bytes an element until the
+ * backward pass instead of x and z:
+ *   fwd: z, mu, rsigma as hk_dropout_add_ln_fwd, (q, scale) = x in 8 bits; x_out (optional): x in rtype, for the
+ *        residual stream.  x_out may be x0 or residual (the same address, pitch and type).
+ *   out: z again, from the kept x (gamma rsigma (x - mu) + beta; RMSNorm: gamma rsigma x), e.g. for the weight
+ *        gradient of the product behind the norm.
+ *   bwd: with x^ = rsigma (x - mu) of the kept x and u = dz gamma:
+ *        dx = rsigma (u - mean(u) - x^ mean(u x^)) + dx_in   (RMSNorm: no mean(u), x^ = rsigma x), written as itype to
+ *        dx0 and, if given, as rtype to dresidual; dgamma = sum dz x^, dbeta = sum dz over the rows.
+ * What is kept is x itself, in steps of 1/64 to 1/128 of the largest magnitude in its block: of a LayerNorm row whose
+ * common offset is far larger than its spread, few bits of x - mu are left.
+ * Types: x0, z, gamma, beta, dz, dx0, dgamma, dbeta itype (fp32 / bf16 / fp16); residual, x_out, dx_in, dresidual
+ * rtype: itype or fp32.  mu, rsigma: fp32 [rows], dense.  residual, gamma, beta, x_out, dx_in, dresidual, dgamma,
+ * dbeta may be NULL; an RMSNorm has no dbeta and its backward reads no mu.  cols <= 32768.  The backward's workspace
+ * (16-byte aligned) serves the column sums; one that is needed for neither may be NULL.  dx0 / dresidual may be dz or
+ * dx_in (the same address, pitch and type). */
+HK_API int hk_add_ln_q8_fwd(int itype, int rtype, const void* x0, int64_t x0_pitch, const void* residual,
+                            int64_t residual_pitch, const void* gamma, const void* beta, void* z,
+                            int64_t z_pitch, void* x_out, int64_t x_out_pitch, int8_t* q, uint8_t* scale,
+                            float* mu, float* rsigma, int64_t rows, int64_t cols, float eps, int is_rms_norm,
+                            hkStream_t stream);
+HK_API int hk_add_ln_q8_out(int itype, const int8_t* q, const uint8_t* scale, const float* mu,
+                            const float* rsigma, const void* gamma, const void* beta, void* z, int64_t z_pitch,
+                            int64_t rows, int64_t cols, int is_rms_norm, hkStream_t stream);
+HK_API int hk_add_ln_q8_bwd_workspace_bytes(int64_t rows, int64_t cols, size_t* bytes);
+HK_API int hk_add_ln_q8_bwd(int itype, int rtype, const void* dz, int64_t dz_pitch, const void* dx_in,
+                            int64_t dx_in_pitch, const int8_t* q, const uint8_t* scale, const float* mu,
+                            const float* rsigma, const void* gamma, void* dx0, int64_t dx0_pitch,
+                            void* dresidual, int64_t dresidual_pitch, void* dgamma, void* dbeta, int64_t rows,
+                            int64_t cols, int is_rms_norm, void* workspace, size_t workspace_bytes,
+                            hkStream_t stream);
+
+/* ======================================================================== *
  * Element-wise operators on dense arrays of fp32 / bf16 / fp16 / fp64 (16-bit
  * floats compute in fp32 and round once).  out may alias an input of its shape.
  *   hk_unary: exp, log, negate, sqrt.  Replaces ExpCuda, LogCuda, OppositeCuda,
