@@ -495,26 +495,34 @@ def vocab_parallel_ce_bwd_fused(logits, labels, lse, grad_loss, out, vocab_start
                                                stream if stream is not None else current_stream()))
 
 
-def _rows_2d(t, name):
-    """(rows, cols, pitch) of a [rows, cols] operand: dense, or a 2-D view with a unit-stride last dimension."""
-    cols = t.shape[-1]
-    return (t.numel() // cols if cols else 0), cols, _pitch(t, cols)
-
-
-def _same(name, want, **tensors):
-    """Refuses operands of another shape than [rows, cols] rows, or of fewer values than `want` asks for."""
-    for what, (t, shape) in tensors.items():
-        if t is not None and tuple(t.shape) != tuple(shape):
-            raise HkError(-1, "%s: %s must have shape %s, got %s" % (name, what, tuple(shape), tuple(t.shape)))
-    for what, t in want:
-        if t is not None and not t.is_contiguous():
-            raise HkError(-1, "%s: %s must be dense" % (name, what))
-
-
-def _typed(name, dtype, **tensors):
-    for what, t in tensors.items():
-        if t is not None and t.dtype != dtype:
+# What follows checks its operands before a call, in hk_call.so; where they do not fit, these say what was wrong.
+def _refuse(name, ref, rows, values=(), operands=()):
+    """Raises for the first operand that does not fit.  ref: the [.., cols] operand the others are measured by; values:
+    (what, tensor, count, dtype), dense; operands: (what, tensor, dtype or None), of ref's shape."""
+    import torch
+    cols = ref.shape[-1] if ref.dim() else 0
+    for what, t in [("operand", ref)] + [(v[0], v[1]) for v in list(values) + list(operands)]:
+        if t is not None and not t.is_cuda:
+            raise HkError(-1, "%s: %s must be on the GPU" % (name, what))
+        if t is not None and t.get_device() != torch.cuda.current_device():
+            raise HkError(-1, "%s: %s is on device %d, the current device is %d" % (name, what, t.get_device(),
+                                                                                   torch.cuda.current_device()))
+    if ref.dim() < 1:
+        raise HkError(-1, "%s: rows are expected, got a scalar" % name)
+    _pitch(ref, cols)
+    for what, t, count, dtype in values:
+        if t is not None and (t.numel() != count or t.dtype != dtype or not t.is_contiguous()):
+            raise HkError(-1, "%s: %s must hold %d values of %s, dense; got shape %s of %s" %
+                          (name, what, count, dtype, tuple(t.shape), t.dtype))
+    for what, t, dtype in operands:
+        if t is None:
+            continue
+        if t.shape[-1:] != ref.shape[-1:] or t.numel() != ref.numel():
+            raise HkError(-1, "%s: %s must have shape %s, got %s" % (name, what, tuple(ref.shape), tuple(t.shape)))
+        if dtype is not None and t.dtype != dtype:
             raise HkError(-1, "%s: %s must be %s, got %s" % (name, what, dtype, t.dtype))
+        _pitch(t, cols)
+    raise HkError(-1, "%s: operands of these types are not taken" % name)
 
 
 def token_logprob_workspace_bytes(dtype, rows, cols, top=0):
@@ -523,13 +531,20 @@ def token_logprob_workspace_bytes(dtype, rows, cols, top=0):
     return n.value
 
 
-def _top(name, top_value, top_token, lead):
-    top = 0 if top_value is None else top_value.shape[-1]
-    if (top_value is None) != (top_token is None):
+def _top(name, value, token):
+    """How many alternatives a pair of tensors holds (none: 0)."""
+    if (value is None) != (token is None):
         raise HkError(-1, "%s: values and tokens of the alternatives come together" % name)
-    _same(name, [("alternatives' values", top_value), ("alternatives' tokens", top_token)],
-          alternatives=(top_value, tuple(lead) + (top,)), tokens=(top_token, tuple(lead) + (top,)))
-    return (None, None, 0) if top == 0 else (top_value, top_token, top)
+    if value is None:
+        return 0
+    if value.dim() < 1 or value.shape != token.shape:
+        raise HkError(-1, "%s: values and tokens of the alternatives differ in shape, %s and %s" %
+                      (name, tuple(value.shape), tuple(token.shape)))
+    return value.shape[-1]
+
+
+def _size(workspace):
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
 
 
 def token_logprob_fwd(logits, tokens, logprob, entropy, lse, top_logprob, top_token, ignored_index, workspace=None,
@@ -537,64 +552,66 @@ def token_logprob_fwd(logits, tokens, logprob, entropy, lse, top_logprob, top_to
     """hk_token_logprob_fwd: logits [..., cols] (dense, or 2-D with a row pitch), tokens int64 with one value a row; logprob,
     entropy, lse fp32 likewise; top_logprob fp32 and top_token int64 [rows, top].  Any output may be None.  Allocates the
     workspace when none is passed, and returns it."""
-    import torch
     n = _call or native()
-    name = "token_logprob_fwd"
-    rows, cols, pitch = _rows_2d(logits, name)
-    _typed(name, torch.int64, tokens=tokens, top_token=top_token)
-    _typed(name, torch.float32, logprob=logprob, entropy=entropy, lse=lse, top_logprob=top_logprob)
-    for what, t in (("tokens", tokens), ("logprob", logprob), ("entropy", entropy), ("lse", lse)):
-        if t is not None and (t.numel() != rows or not t.is_contiguous()):
-            raise HkError(-1, "%s: %s must hold one value per row, dense" % (name, what))
-    value, token, top = _top(name, top_logprob, top_token, (rows,))
-    code = dtype_code(logits)
+    top = _top("token_logprob_fwd", top_logprob, top_token)
+    ref = n.row_operand(logits)
+    if ref is not None:
+        rows, cols, pitch, code, dev = ref
+    if ref is None or not (n.values(rows, 4, dev, tokens) and n.values(rows, 6, dev, logprob, entropy, lse) and
+                           n.values(rows * top, 6, dev, top_logprob) and n.values(rows * top, 4, dev, top_token)):
+        import torch
+        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        _refuse("token_logprob_fwd", logits, rows, [
+            ("tokens", tokens, rows, torch.int64), ("logprob", logprob, rows, torch.float32),
+            ("entropy", entropy, rows, torch.float32), ("lse", lse, rows, torch.float32),
+            ("top_logprob", top_logprob, rows * top, torch.float32), ("top_token", top_token, rows * top, torch.int64)])
     if workspace is None and rows:
         workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top), logits.device)
-    wsb = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    check(n.hk_token_logprob_fwd(code, logits, pitch, tokens, logprob, entropy, lse, value, token, top, rows, cols,
-                                 int(ignored_index), workspace, wsb, stream))
+    check(n.hk_token_logprob_fwd(code, logits, pitch, tokens, logprob, entropy, lse, top_logprob, top_token, top, rows, cols,
+                                 ignored_index, workspace, _size(workspace), stream))
     return workspace
 
 
 def token_logprob_bwd(logits, tokens, lse, entropy, grad_logprob, grad_entropy, dlogits, ignored_index, vocab_start=0,
                       stream=None):
     """hk_token_logprob_bwd; grad_logprob or grad_entropy (fp32, one value a row) may be None, entropy with grad_entropy."""
-    import torch
     n = _call or native()
-    name = "token_logprob_bwd"
-    rows, cols, pitch = _rows_2d(logits, name)
-    _same(name, [], dlogits=(dlogits, logits.shape))
-    _typed(name, logits.dtype, dlogits=dlogits)
-    _typed(name, torch.int64, tokens=tokens)
-    _typed(name, torch.float32, lse=lse, entropy=entropy, grad_logprob=grad_logprob, grad_entropy=grad_entropy)
-    for what, t in (("tokens", tokens), ("lse", lse), ("entropy", entropy), ("grad_logprob", grad_logprob),
-                    ("grad_entropy", grad_entropy)):
-        if t is not None and (t.numel() != rows or not t.is_contiguous()):
-            raise HkError(-1, "%s: %s must hold one value per row, dense" % (name, what))
-    check(n.hk_token_logprob_bwd(dtype_code(logits), logits, pitch, tokens, lse, entropy, grad_logprob, grad_entropy, dlogits,
-                                 _pitch(dlogits, cols), rows, cols, int(vocab_start), int(ignored_index), stream))
+    ref = n.row_operand(logits)
+    out = None
+    if ref is not None:
+        rows, cols, pitch, code, dev = ref
+        out = n.row_pitches(rows, cols, code, dev, dlogits)
+    if out is None or not (n.values(rows, 4, dev, tokens) and n.values(rows, 6, dev, lse, entropy, grad_logprob, grad_entropy)):
+        import torch
+        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        _refuse("token_logprob_bwd", logits, rows, [
+            ("tokens", tokens, rows, torch.int64), ("lse", lse, rows, torch.float32), ("entropy", entropy, rows, torch.float32),
+            ("grad_logprob", grad_logprob, rows, torch.float32), ("grad_entropy", grad_entropy, rows, torch.float32)],
+            [("dlogits", dlogits, logits.dtype)])
+    check(n.hk_token_logprob_bwd(code, logits, pitch, tokens, lse, entropy, grad_logprob, grad_entropy, dlogits, out[0], rows,
+                                 cols, vocab_start, ignored_index, stream))
 
 
 def vocab_parallel_logprob_stats(logits, tokens, stats, top_value, top_token, vocab_start, ignored_index, workspace=None,
                                  stream=None):
     """hk_vocab_parallel_logprob_stats: stats fp32 [4, rows], top_value fp32 and top_token int64 [rows, top] (or None) of this
     column shard."""
-    import torch
     n = _call or native()
-    name = "vocab_parallel_logprob_stats"
-    rows, cols, pitch = _rows_2d(logits, name)
-    _typed(name, torch.int64, tokens=tokens, top_token=top_token)
-    _typed(name, torch.float32, stats=stats, top_value=top_value)
-    _same(name, [("stats", stats), ("tokens", tokens)], stats=(stats, (4, rows)))
-    if tokens.numel() != rows:
-        raise HkError(-1, "%s: tokens must hold one value per row" % name)
-    value, token, top = _top(name, top_value, top_token, (rows,))
-    code = dtype_code(logits)
+    top = _top("vocab_parallel_logprob_stats", top_value, top_token)
+    ref = n.row_operand(logits)
+    if ref is not None:
+        rows, cols, pitch, code, dev = ref
+    if ref is None or not (n.values(rows, 4, dev, tokens) and n.values(4 * rows, 6, dev, stats) and
+                           n.values(rows * top, 6, dev, top_value) and n.values(rows * top, 4, dev, top_token)):
+        import torch
+        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        _refuse("vocab_parallel_logprob_stats", logits, rows, [
+            ("tokens", tokens, rows, torch.int64), ("stats", stats, 4 * rows, torch.float32),
+            ("top_value", top_value, rows * top, torch.float32), ("top_token", top_token, rows * top, torch.int64)])
     if workspace is None and rows:
         workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top), logits.device)
-    wsb = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    check(n.hk_vocab_parallel_logprob_stats(code, logits, pitch, tokens, stats, value, token, top, rows, cols,
-                                            int(vocab_start), int(ignored_index), workspace, wsb, stream))
+    check(n.hk_vocab_parallel_logprob_stats(code, logits, pitch, tokens, stats, top_value, top_token, top, rows, cols,
+                                            vocab_start, ignored_index, workspace, _size(workspace), stream))
     return workspace
 
 
@@ -602,23 +619,28 @@ def vocab_parallel_logprob_combine(stats, top_values, top_tokens, tokens, ignore
                                    top_token, vocab_size=-1, stream=None):
     """hk_vocab_parallel_logprob_combine: stats fp32 [shards, 4, rows], top_values fp32 and top_tokens int64 [shards, rows, top]
     (or None) -> the outputs of token_logprob_fwd."""
-    import torch
     n = _call or native()
     name = "vocab_parallel_logprob_combine"
-    shards, _, rows = stats.shape
-    _typed(name, torch.int64, tokens=tokens, top_tokens=top_tokens, top_token=top_token)
-    _typed(name, torch.float32, stats=stats, top_values=top_values, top_logprob=top_logprob, logprob=logprob, entropy=entropy,
-           lse=lse)
-    _same(name, [("stats", stats)], stats=(stats, (shards, 4, rows)))
-    for what, t in (("tokens", tokens), ("logprob", logprob), ("entropy", entropy), ("lse", lse)):
-        if t is not None and (t.numel() != rows or not t.is_contiguous()):
-            raise HkError(-1, "%s: %s must hold one value per row, dense" % (name, what))
-    values, numbers, given = _top(name, top_values, top_tokens, (shards, rows))
-    value, token, top = _top(name, top_logprob, top_token, (rows,))
+    given, top = _top(name, top_values, top_tokens), _top(name, top_logprob, top_token)
     if given != top:
         raise HkError(-1, "%s: the shards hold %d alternatives, %d are asked for" % (name, given, top))
-    check(n.hk_vocab_parallel_logprob_combine(stats, values, numbers, shards, tokens, int(ignored_index), int(vocab_size),
-                                              logprob, entropy, lse, value, token, top, rows, stream))
+    shards, four, rows = stats.shape
+    dev = stats.get_device()
+    if not (four == 4 and n.row_operand(stats) and n.values(4 * shards * rows, 6, dev, stats) and n.values(rows, 4, dev, tokens) and
+            n.values(rows, 6, dev, logprob, entropy, lse) and n.values(rows * top, 6, dev, top_logprob) and
+            n.values(rows * top, 4, dev, top_token) and n.values(shards * rows * top, 6, dev, top_values) and
+            n.values(shards * rows * top, 4, dev, top_tokens)):
+        import torch
+        if four != 4:
+            raise HkError(-1, "%s: stats must have shape [shards, 4, rows], got %s" % (name, tuple(stats.shape)))
+        _refuse(name, stats, rows, [
+            ("stats", stats, 4 * shards * rows, torch.float32), ("tokens", tokens, rows, torch.int64),
+            ("logprob", logprob, rows, torch.float32), ("entropy", entropy, rows, torch.float32),
+            ("lse", lse, rows, torch.float32), ("top_logprob", top_logprob, rows * top, torch.float32),
+            ("top_token", top_token, rows * top, torch.int64), ("top_values", top_values, shards * rows * top, torch.float32),
+            ("top_tokens", top_tokens, shards * rows * top, torch.int64)])
+    check(n.hk_vocab_parallel_logprob_combine(stats, top_values, top_tokens, shards, tokens, ignored_index, vocab_size,
+                                              logprob, entropy, lse, top_logprob, top_token, top, rows, stream))
 
 
 Q8_BLOCK = 32
@@ -632,74 +654,80 @@ def q8_empty(rows, cols, device):
             torch.empty((rows, blocks), dtype=torch.uint8, device=device))
 
 
-def _q8_pair(name, q, scale, rows, cols):
+def _q8_values(q, scale, rows, cols):
     import torch
-    blocks = (cols + Q8_BLOCK - 1) // Q8_BLOCK
-    _typed(name, torch.int8, q=q)
-    _typed(name, torch.uint8, scale=scale)
-    _same(name, [("q", q), ("scale", scale)], q=(q, (rows, blocks * Q8_BLOCK)), scale=(scale, (rows, blocks)))
+    blocks = rows * ((cols + Q8_BLOCK - 1) // Q8_BLOCK)
+    return [("q", q, blocks * Q8_BLOCK, torch.int8), ("scale", scale, blocks, torch.uint8)]
 
 
 def q8_pack(x, q, scale, stream=None):
     """hk_q8_pack: x [..., cols] fp32 / bf16 / fp16 (dense, or 2-D with a row pitch) -> q int8 [rows, blocks * 32] and scale
     uint8 [rows, blocks]."""
     n = _call or native()
-    rows, cols, pitch = _rows_2d(x, "q8_pack")
-    _q8_pair("q8_pack", q, scale, rows, cols)
-    check(n.hk_q8_pack(dtype_code(x), x, pitch, q, scale, rows, cols, stream))
+    ref = n.row_operand(x)
+    if ref is not None:
+        rows, cols, pitch, code, dev = ref
+        blocks = rows * ((cols + 31) >> 5)
+    if ref is None or not (n.values(blocks * 32, 1, dev, q) and n.values(blocks, 0, dev, scale)):
+        rows = x.numel() // x.shape[-1] if x.numel() else 0
+        _refuse("q8_pack", x, rows, _q8_values(q, scale, rows, x.shape[-1]))
+    check(n.hk_q8_pack(code, x, pitch, q, scale, rows, cols, stream))
 
 
 def q8_unpack(q, scale, out, stream=None):
     n = _call or native()
-    rows, cols, pitch = _rows_2d(out, "q8_unpack")
-    _q8_pair("q8_unpack", q, scale, rows, cols)
-    check(n.hk_q8_unpack(dtype_code(out), q, scale, out, pitch, rows, cols, stream))
+    ref = n.row_operand(out)
+    if ref is not None:
+        rows, cols, pitch, code, dev = ref
+        blocks = rows * ((cols + 31) >> 5)
+    if ref is None or not (n.values(blocks * 32, 1, dev, q) and n.values(blocks, 0, dev, scale)):
+        rows = out.numel() // out.shape[-1] if out.numel() else 0
+        _refuse("q8_unpack", out, rows, _q8_values(q, scale, rows, out.shape[-1]))
+    check(n.hk_q8_unpack(code, q, scale, out, pitch, rows, cols, stream))
 
 
-def _q8_norm_operands(name, ref, stats, params, same, residuals):
-    """Refuses what the C entry points cannot see: shapes and types beside the one dtype code they are given."""
+def _q8_norm(n, name, ref, q, scale, stats, params, same, residuals):
+    """(rows, cols, dtype code, rtype code, pitches of ref, same and residuals) of a norm's operands."""
+    got = n.row_operand(ref)
+    if got is not None:
+        rows, cols, pitch, code, dev = got
+        blocks = rows * ((cols + 31) >> 5)
+        rcode = code
+        for t in residuals:
+            if t is not None:
+                rcode = dtype_code(t)
+        a = n.row_pitches(rows, cols, code, dev, *same)
+        b = n.row_pitches(rows, cols, rcode, dev, *residuals)
+        if (a is not None and b is not None and n.values(blocks * 32, 1, dev, q) and n.values(blocks, 0, dev, scale) and
+                n.values(rows, 6, dev, *stats) and n.values(cols, code, dev, *params)):
+            return rows, cols, code, rcode, pitch, a, b
     import torch
-    cols = ref.shape[-1]
+    cols = ref.shape[-1] if ref.dim() else 0
     rows = ref.numel() // cols if cols else 0
-    for what, t in stats:
-        if t is not None and (t.numel() != rows or t.dtype != torch.float32 or not t.is_contiguous()):
-            raise HkError(-1, "%s: %s must hold one fp32 value per row, dense" % (name, what))
-    for what, t in params:
-        if t is not None and (tuple(t.shape) != (cols,) or t.dtype != ref.dtype or not t.is_contiguous()):
-            raise HkError(-1, "%s: %s must hold one %s value per column, dense" % (name, what, ref.dtype))
-    for what, t in same + residuals:
-        if t is not None and t.shape != ref.shape:
-            raise HkError(-1, "%s: %s must have shape %s, got %s" % (name, what, tuple(ref.shape), tuple(t.shape)))
-    for what, t in same:
-        if t is not None and t.dtype != ref.dtype:
-            raise HkError(-1, "%s: %s must be %s, got %s" % (name, what, ref.dtype, t.dtype))
-    types = {t.dtype for _, t in residuals if t is not None}
+    types = {t.dtype for t in residuals if t is not None}
     if len(types) > 1:
-        raise HkError(-1, "%s: %s must be of one type" % (name, " and ".join(what for what, _ in residuals)))
-    return rows, cols, _dtype_codes()[types.pop()] if types else dtype_code(ref)
+        raise HkError(-1, "%s: the residual stream's operands must be of one type, got %s" % (name, sorted(map(str, types))))
+    _refuse(name, ref, rows, _q8_values(q, scale, rows, cols) +
+            [("a row statistic", t, rows, torch.float32) for t in stats] +
+            [("a parameter or its gradient", t, cols, ref.dtype) for t in params],
+            [("an operand", t, ref.dtype) for t in same] + [("an operand of the residual stream", t, None) for t in residuals])
 
 
 def add_ln_q8_fwd(x0, residual, gamma, beta, z, x_out, q, scale, mu, rsigma, eps, is_rms, stream=None):
     """hk_add_ln_q8_fwd: the norm of x0 + residual, whose sum is kept in (q, scale); residual and x_out (rtype: x0's type or
     fp32), gamma and beta may be None."""
     n = _call or native()
-    name = "add_ln_q8_fwd"
-    rows, cols, rtype = _q8_norm_operands(name, x0, [("mu", mu), ("rsigma", rsigma)], [("gamma", gamma), ("beta", beta)],
-                                          [("z", z)], [("residual", residual), ("x_out", x_out)])
-    _q8_pair(name, q, scale, rows, cols)
-    check(n.hk_add_ln_q8_fwd(dtype_code(x0), rtype, x0, _pitch(x0, cols), residual, _pitch(residual, cols), gamma, beta, z,
-                             _pitch(z, cols), x_out, _pitch(x_out, cols), q, scale, mu, rsigma, rows, cols, float(eps),
-                             int(is_rms), stream))
+    rows, cols, code, rcode, xp, (zp,), (rp, op) = _q8_norm(n, "add_ln_q8_fwd", x0, q, scale, (mu, rsigma), (gamma, beta), (z,),
+                                                            (residual, x_out))
+    check(n.hk_add_ln_q8_fwd(code, rcode, x0, xp, residual, rp, gamma, beta, z, zp, x_out, op, q, scale, mu, rsigma, rows, cols,
+                             eps, int(is_rms), stream))
 
 
 def add_ln_q8_out(q, scale, mu, rsigma, gamma, beta, z, is_rms, stream=None):
     """hk_add_ln_q8_out: z of a norm again, from its kept input."""
     n = _call or native()
-    name = "add_ln_q8_out"
-    rows, cols, _ = _q8_norm_operands(name, z, [("mu", mu), ("rsigma", rsigma)], [("gamma", gamma), ("beta", beta)], [], [])
-    _q8_pair(name, q, scale, rows, cols)
-    check(n.hk_add_ln_q8_out(dtype_code(z), q, scale, mu, rsigma, gamma, beta, z, _pitch(z, cols), rows, cols, int(is_rms),
-                             stream))
+    rows, cols, code, _, zp, _, _ = _q8_norm(n, "add_ln_q8_out", z, q, scale, (mu, rsigma), (gamma, beta), (), ())
+    check(n.hk_add_ln_q8_out(code, q, scale, mu, rsigma, gamma, beta, z, zp, rows, cols, int(is_rms), stream))
 
 
 def add_ln_q8_bwd_workspace_bytes(rows, cols):
@@ -712,17 +740,12 @@ def add_ln_q8_bwd(dz, dx_in, q, scale, mu, rsigma, gamma, dx0, dresidual, dgamma
     """hk_add_ln_q8_bwd; dx_in and dresidual (rtype: dz's type or fp32), gamma, dgamma, dbeta may be None.  Allocates the
     workspace when none is passed, and returns it."""
     n = _call or native()
-    name = "add_ln_q8_bwd"
-    rows, cols, rtype = _q8_norm_operands(name, dz, [("mu", mu), ("rsigma", rsigma)],
-                                          [("gamma", gamma), ("dgamma", dgamma), ("dbeta", dbeta)], [("dx0", dx0)],
-                                          [("dx_in", dx_in), ("dresidual", dresidual)])
-    _q8_pair(name, q, scale, rows, cols)
+    rows, cols, code, rcode, zp, (xp,), (ip, rp) = _q8_norm(n, "add_ln_q8_bwd", dz, q, scale, (mu, rsigma),
+                                                            (gamma, dgamma, dbeta), (dx0,), (dx_in, dresidual))
     if workspace is None and (dgamma is not None or dbeta is not None):
         workspace = _workspace(add_ln_q8_bwd_workspace_bytes(rows, cols), dz.device)
-    wsb = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    check(n.hk_add_ln_q8_bwd(dtype_code(dz), rtype, dz, _pitch(dz, cols), dx_in, _pitch(dx_in, cols), q, scale, mu, rsigma,
-                             gamma, dx0, _pitch(dx0, cols), dresidual, _pitch(dresidual, cols), dgamma, dbeta, rows, cols,
-                             int(is_rms), workspace, wsb, stream))
+    check(n.hk_add_ln_q8_bwd(code, rcode, dz, zp, dx_in, ip, q, scale, mu, rsigma, gamma, dx0, xp, dresidual, rp, dgamma, dbeta,
+                             rows, cols, int(is_rms), workspace, _size(workspace), stream))
     return workspace
 
 

@@ -14,53 +14,77 @@
 namespace hk {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
 // differences of logits are cut here where they enter a product: exp() of it is 0, and 0 * -inf would be NaN
 constexpr float kFarBelow = -1e4f;
 constexpr int kMaxTop = 32;          // alternatives of a row
 constexpr int kMaxShards = 64;       // lists that one wavefront merges
+constexpr int kMaxSplits = 8;        // parts of a row
 constexpr int kMaxCandidates = 512;
 
-struct LogprobTuple {   // (m, S, W)
+// (m, S, W) of some elements, S and W taken in the log2 domain against M = fl(m log2(e)): S = sum 2^t, W = sum 2^t t with
+// t = x log2(e) - M, one multiply-add per element.  The rounding of M is common to all of them and drops out of what is
+// made of S and W; towards other (m, S, W), t moves by a difference of two Ms.
+struct LogprobTuple {
   static constexpr int K = 3;
   float v[3];
   static __device__ __forceinline__ LogprobTuple identity() { return LogprobTuple{{kNegInf, 0.f, 0.f}}; }
-  static __device__ __forceinline__ float finite_or_zero(float m) { return m == kNegInf ? 0.f : m; }
-  // this relative to the maximum mg (finite; or +inf, which ends in NaN)
-  __device__ __forceinline__ void rebase(float mg) {
-    const float d = fmaxf(v[0] - mg, kFarBelow), f = __builtin_amdgcn_exp2f(d * kLog2e);
+  // (finite below: an empty maximum; a maximum whose M is past the range of fp32 on either side goes to row_max_count)
+  static __device__ __forceinline__ float base(float m) { return fmaxf(m * kLog2e, -kLog2Bound); }
+  __device__ __forceinline__ void rebase(float from, float to) {
+    const float d = fmaxf(from - to, kFarBelow), f = __builtin_amdgcn_exp2f(d);
     v[2] = f * fmaf(d, v[1], v[2]);
     v[1] *= f;
   }
   static __device__ __forceinline__ LogprobTuple merge(LogprobTuple a, LogprobTuple b) {
-    const float m = fmaxf(a.v[0], b.v[0]), mg = finite_or_zero(m);
-    a.rebase(mg);
-    b.rebase(mg);
+    const float m = fmaxf(a.v[0], b.v[0]), to = base(m);
+    a.rebase(base(a.v[0]), to);
+    b.rebase(base(b.v[0]), to);
     return LogprobTuple{{m, a.v[1] + b.v[1], a.v[2] + b.v[2]}};
   }
-  // N more elements, taken against the new maximum
+  // N more elements, whose maximum is m
   template <int N>
-  __device__ __forceinline__ void add(const float* f) {
-    float m = v[0];
-    if constexpr (N == 1) {
-      m = fmaxf(m, f[0]);
-    } else {
-      static_assert(N % 2 == 0, "pairs of elements per max3");
-#pragma unroll
-      for (int e = 0; e < N; e += 2) m = max3(m, f[e], f[e + 1]);
-    }
-    const float mg = finite_or_zero(m);
-    rebase(mg);
+  __device__ __forceinline__ void add(const float* f, float m) {
+    m = fmaxf(v[0], m);
+    const float to = base(m);
+    rebase(base(v[0]), to);
     v[0] = m;
     float s[2] = {v[1], 0.f}, w[2] = {v[2], 0.f};
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float d = f[e] - mg, x = __builtin_amdgcn_exp2f(d * kLog2e);
+      const float t = fmaf(f[e], kLog2e, -to), x = __builtin_amdgcn_exp2f(t);
       s[e & 1] += x;
-      w[e & 1] = fmaf(x, fmaxf(d, kFarBelow), w[e & 1]);
+      w[e & 1] = fmaf(x, fmaxf(t, kFarBelow), w[e & 1]);
     }
     v[1] = s[0] + s[1];
     v[2] = w[0] + w[1];
+  }
+};
+template <int N>
+__device__ __forceinline__ float max_of(const float* f) {
+  static_assert(N % 2 == 0, "pairs of elements per max3");
+  float m = fmaxf(f[0], f[1]);
+#pragma unroll
+  for (int e = 2; e < N; e += 2) m = max3(m, f[e], f[e + 1]);
+  return m;
+}
+
+// (m, S, W) as they go from device to device: S and W against m itself
+struct LogprobStats {
+  static constexpr int K = 3;
+  float v[3];
+  static __device__ __forceinline__ LogprobStats identity() { return LogprobStats{{kNegInf, 0.f, 0.f}}; }
+  __device__ __forceinline__ void rebase(float to) {   // to: finite, or +inf, which ends in NaN
+    const float d = fmaxf(v[0] - to, kFarBelow), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    v[2] = f * fmaf(d, v[1], v[2]);
+    v[1] *= f;
+  }
+  static __device__ __forceinline__ LogprobStats merge(LogprobStats a, LogprobStats b) {
+    const float m = fmaxf(a.v[0], b.v[0]), to = m == kNegInf ? 0.f : m;
+    a.rebase(to);
+    b.rebase(to);
+    return LogprobStats{{m, a.v[1] + b.v[1], a.v[2] + b.v[2]}};
   }
 };
 
@@ -106,13 +130,29 @@ struct PartSpan {
   __device__ __forceinline__ u32x4 load_again(int v) const { return ld16_keep(row + column(v)); }
 };
 
+// Alternatives.  While the row streams by, a thread writes down the maximum of every few of its vectors.  Then the k-th
+// largest of 64 groups' maxima (group l: lane l of every wavefront) is a lower bound of the row's k-th largest value; its
+// leading bits are found by bisection.  The runs of vectors whose maximum reaches it, some k + k^2 / 128 of them, are shared
+// out over the workgroup and read again, a vector a lane, all at once; elements that reach the bound become candidates, in
+// any order, and a candidate's place is the number of candidates before it.
+constexpr int kMaxSlots = 8;          // runs of vectors of a thread
+constexpr int kMaxRuns = 256;
+struct TopShared {
+  __align__(16) uint32_t key[kMaxCandidates];
+  __align__(16) int col[kMaxCandidates];
+  float lane_max[8][kWave];           // of at most 512 threads
+  uint16_t run[kMaxRuns];             // slot * 1024 + thread
+  uint32_t runs, count;
+};
+
 // MODE 0: one workgroup per row, final values.  MODE 1: workgroup (part, row) leaves the statistics and the alternatives
 // of a part of the row.  TOP: with alternatives.
 template <typename T, bool RAGGED, int MODE, bool TOP>
-__global__ __launch_bounds__(1024, 8)
+__global__ __launch_bounds__(512, 8)
 void token_logprob_kernel(LogprobArgs a) {
   constexpr int VEC = VecIO<T>::N, U = sizeof(T) == 2 ? 4 : 8;
   __shared__ float red[kMaxWaves * 3];
+  extern __shared__ __align__(16) float run_max[];   // TOP: [slots][threads]
   const int t = int(threadIdx.x), threads = a.threads, nwaves = threads >> 6;
   const int row = MODE ? int(blockIdx.y) : int(blockIdx.x);
   float* const top_value = TOP ? a.top_value + ((MODE ? int64_t(blockIdx.x) * a.rows : 0) + row) * a.top : nullptr;
@@ -147,66 +187,104 @@ void token_logprob_kernel(LogprobArgs a) {
   if constexpr (RAGGED) {
     if (span.edge >= 0) edge = Cvt<T>::load(xr + span.edge);
   }
+  // rounds of U vectors a thread, `per_slot` of which share a maximum
+  const int round = U * threads;
+  [[maybe_unused]] const int per_slot = TOP ? (span.nvec + round * kMaxSlots - 1) / (round * kMaxSlots) : 0;
+  [[maybe_unused]] int slot = 0, in_slot = 0;
+  [[maybe_unused]] float cur = kNegInf;
+  auto note = [&](float m) {
+    if constexpr (TOP) {
+      cur = fmaxf(cur, m);
+      if (++in_slot == per_slot) {   // uniform
+        run_max[slot++ * threads + t] = cur;
+        in_slot = 0;
+        cur = kNegInf;
+      }
+    }
+  };
   int v = 0;
 #pragma nounroll
-  for (; v + U * threads <= span.nvec; v += U * threads) {
+  for (; v + round <= span.nvec; v += round) {
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = span.load(v + u * threads + t);
     float f[U * VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) VecIO<T>::unpack(raw[u], &f[u * VEC]);
-    p.template add<U * VEC>(f);
+    const float m = max_of<U * VEC>(f);
+    p.template add<U * VEC>(f, m);
+    note(m);
   }
-  if (v < span.nvec) {
+  if (v < span.nvec) {   // what is left, a vector a thread at a time
     u32x4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       raw[u] = neg_inf_vec<T>();
       if (v + u * threads + t < span.nvec) raw[u] = span.load(v + u * threads + t);
     }
-    float f[U * VEC];
+    float most = kNegInf;
+    if (v + (U - 1) * threads < span.nvec) {   // uniform: all of them in some thread
+      float f[U * VEC];
 #pragma unroll
-    for (int u = 0; u < U; ++u) VecIO<T>::unpack(raw[u], &f[u * VEC]);
-    p.template add<U * VEC>(f);
+      for (int u = 0; u < U; ++u) VecIO<T>::unpack(raw[u], &f[u * VEC]);
+      most = max_of<U * VEC>(f);
+      p.template add<U * VEC>(f, most);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u) {
+        if (v + u * threads < span.nvec) {   // uniform
+          float f[VEC];
+          VecIO<T>::unpack(raw[u], f);
+          const float m = max_of<VEC>(f);
+          p.template add<VEC>(f, m);
+          most = fmaxf(most, m);
+        }
+      }
+    }
+    note(most);
   }
-  if constexpr (RAGGED) p.template add<1>(&edge);
+  if constexpr (TOP) {
+    if (in_slot) run_max[slot++ * threads + t] = cur;   // uniform
+  }
+  if constexpr (RAGGED) p.template add<1>(&edge, edge);
 
   [[maybe_unused]] const float mine = p.v[0];   // the maximum of this thread's elements
   p = group_allreduce_tuple(p, red, 0, nwaves);
-  const float log_s = logf(p.v[1]), lse = p.v[0] + log_s;
+  float m = p.v[0], s = p.v[1], w = p.v[2], off = 0.f;   // off: the rounding of M
+  if (__builtin_expect(m != kNegInf && !(fabsf(m * kLog2e) < kLog2Bound), 0)) {   // uniform; a NaN is none
+    s = row_max_count<T>(xr, cols, t, threads, [&](auto x) { __syncthreads(); return group_allreduce_tuple(x, red, 0, nwaves); }, m);
+    w = 0.f;
+  } else if (m != kNegInf) {
+    off = fmaf(m, kLog2e, -LogprobTuple::base(m));
+  }
+  const float log_s = logf(s) - off * kLn2, lse = m + log_s;
   if (t == 0) {
     const int64_t local = token - a.vocab_start - first;
     const bool inside = local >= 0 && local < cols;
     const float picked = inside ? Cvt<T>::load(xr + local) : 0.f;
     if constexpr (MODE) {
-      stats[0] = p.v[0];
-      stats[a.rows] = p.v[1];
-      stats[2 * int64_t(a.rows)] = p.v[2];
+      const float f = __builtin_amdgcn_exp2f(-off);
+      stats[0] = m;
+      stats[a.rows] = s * f;
+      stats[2 * int64_t(a.rows)] = kLn2 * f * fmaf(-off, s, w);
       stats[3 * int64_t(a.rows)] = picked;
     } else {
-      if (a.logprob) a.logprob[row] = inside ? (picked - p.v[0]) - log_s : __builtin_nanf("");
-      if (a.entropy) a.entropy[row] = log_s - p.v[2] / p.v[1];
+      // m - picked first: the difference of two logits is (nearly) exact however large their common offset is
+      if (a.logprob) a.logprob[row] = inside ? (picked - m) - log_s : __builtin_nanf("");
+      if (a.entropy) a.entropy[row] = logf(s) - kLn2 * (w / s);
       if (a.lse) a.lse[row] = lse;
     }
   }
 
   if constexpr (TOP) {
-    // The k-th largest of 64 groups' maxima (lane l of every wavefront) is a lower bound of the row's k-th largest value:
-    // its leading bits by bisection.  The threads whose maximum reaches it read their elements again and put those that
-    // reach it into a list, some k + k^2 / 128 of them in any order; a candidate's place in the order is the number of
-    // candidates before it.
     constexpr int kBits = sizeof(T) == 4 ? 24 : std::is_same<T, bf16>::value ? 16 : 20;
-    __shared__ float lane_max[kMaxWaves][kWave];
-    __shared__ uint32_t cand_key[kMaxCandidates];
-    __shared__ int cand_col[kMaxCandidates];
-    __shared__ uint32_t count;
+    __shared__ TopShared sh;
     const int lane = t & 63;
-    lane_max[t >> 6][lane] = mine;
-    if (t == 0) count = 0;
+    sh.lane_max[t >> 6][lane] = mine;
+    if (t == 0) sh.runs = sh.count = 0;
     __syncthreads();
     float g = kNegInf;
-    for (int w = 0; w < nwaves; ++w) g = fmaxf(g, lane_max[w][lane]);
+    for (int i = 0; i < nwaves; ++i) g = fmaxf(g, sh.lane_max[i][lane]);
     const uint32_t gk = order_key(g);
     uint32_t bound = 0;
 #pragma unroll
@@ -215,29 +293,57 @@ void token_logprob_kernel(LogprobArgs a) {
       if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(gk >= at)) >= int(a.top)) bound = at;
     }
     bound = max(bound, kKeyNegInf + 1);          // an element of -inf is no alternative
-    auto offer = [&](float f, int col) {
-      const uint32_t k = order_key(f);
-      if (k >= bound && f == f) {
-        const uint32_t i = atomicAdd(&count, 1u);   // the order does not matter
-        if (i < kMaxCandidates) { cand_key[i] = k; cand_col[i] = col; }
-      }
-    };
-    auto each = [&](auto fn) {   // fn(element, column in the part) over this thread's elements
-      for (int w = t; w < span.nvec; w += threads) {
-        float f[VEC];
-        VecIO<T>::unpack(span.load_again(w), f);
+    // (places in the lists: one atomic a thread, whatever it has to put there; their order does not matter)
+    auto offer = [&](auto elements, const float* f, int col) {
+      constexpr int N = decltype(elements)::value;
+      uint32_t k[N];
+      int n = 0;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) fn(f[j], span.column(w) + j);
+      for (int j = 0; j < N; ++j) {
+        k[j] = f[j] == f[j] ? order_key(f[j]) : 0u;
+        n += k[j] >= bound ? 1 : 0;
       }
-      if (RAGGED && span.edge >= 0) fn(edge, span.edge);
+      if (n == 0) return;
+      uint32_t i = atomicAdd(&sh.count, uint32_t(n));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k[j] >= bound) {
+          if (i < kMaxCandidates) { sh.key[i] = k[j]; sh.col[i] = col + j; }
+          ++i;
+        }
     };
-    if (order_key(mine) >= bound) each(offer);
+    if (order_key(mine) >= bound) {
+      uint32_t reach = 0;
+#pragma unroll
+      for (int i = 0; i < kMaxSlots; ++i)
+        if (i < slot && order_key(run_max[i * threads + t]) >= bound) reach |= 1u << i;
+      if (reach) {
+        uint32_t r = atomicAdd(&sh.runs, uint32_t(__builtin_popcount(reach)));
+        for (; reach; reach &= reach - 1, ++r)
+          if (r < kMaxRuns) sh.run[r] = uint16_t(__builtin_ctz(reach) * 1024 + t);
+      }
+      if (RAGGED && span.edge >= 0) offer(std::integral_constant<int, 1>{}, &edge, span.edge);
+    }
     __syncthreads();
-    const int n = int(count);
+    const int runs = int(sh.runs);
+    if (runs <= kMaxRuns) {
+      const int each = per_slot * U;   // vectors of a run
+      for (int i = t; i < runs * each; i += threads) {
+        const int r = i / each, k = i - r * each, at = sh.run[r];
+        const int vec = ((at >> 10) * each + k) * threads + (at & 1023);
+        if (vec < span.nvec) {
+          float f[VEC];
+          VecIO<T>::unpack(span.load_again(vec), f);
+          offer(std::integral_constant<int, VEC>{}, f, span.column(vec));
+        }
+      }
+    }
+    __syncthreads();
+    const int n = int(sh.count);
     const bool none = MODE == 0 && !(fabsf(lse) < __builtin_huge_valf());   // no probabilities: no alternatives
     const float base = MODE ? 0.f : lse;
     const int64_t number0 = a.vocab_start + first;
-    if (t < a.top && (none || t >= n)) {
+    if (t < a.top && (none || (t >= n && runs <= kMaxRuns))) {
       top_value[t] = none ? __builtin_nanf("") : kNegInf;
       top_token[t] = -1;
     }
@@ -247,12 +353,16 @@ void token_logprob_kernel(LogprobArgs a) {
       top_value[place] = f - base;
       top_token[place] = number0 + col;
     };
-    if (n <= kMaxCandidates) {
+    if (n <= kMaxCandidates && runs <= kMaxRuns) {
       for (int i = t; i < n; i += threads) {
-        const uint32_t k = cand_key[i];
-        const int c = cand_col[i];
+        const uint32_t k = sh.key[i];
+        const int c = sh.col[i];
         int place = 0;
-        for (int j = 0; j < n; ++j) place += (cand_key[j] > k || (cand_key[j] == k && cand_col[j] < c)) ? 1 : 0;
+        for (int j = 0; j < n; j += 4) {   // four at a time; what stands behind the n-th is not counted
+          const u32x4 ks = *reinterpret_cast<const u32x4*>(&sh.key[j]), cs = *reinterpret_cast<const u32x4*>(&sh.col[j]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) place += (j + q < n && (ks[q] > k || (ks[q] == k && int(cs[q]) < c))) ? 1 : 0;
+        }
         if (place < a.top) put(place, k, c);
       }
       return;
@@ -264,20 +374,27 @@ void token_logprob_kernel(LogprobArgs a) {
     for (int place = 0; place < a.top; ++place) {
       uint32_t best = 0;
       int best_col = 0x7fffffff;
-      each([&](float f, int col) {
+      auto look = [&](float f, int col) {
         const uint32_t k = order_key(f);
         const bool behind = k < last_key || (k == last_key && col > last_col);
         if (f == f && behind && (k > best || (k == best && col < best_col))) { best = k; best_col = col; }
-      });
-      __syncthreads();   // count, the candidates and the last round's result are read
-      if (t == 0) { count = 0; cand_col[0] = 0x7fffffff; }
+      };
+      for (int i = t; i < span.nvec; i += threads) {
+        float f[VEC];
+        VecIO<T>::unpack(span.load_again(i), f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) look(f[j], span.column(i) + j);
+      }
+      if (RAGGED && span.edge >= 0) look(edge, span.edge);
+      __syncthreads();   // the count, the candidates and the last round's result have been read
+      if (t == 0) { sh.count = 0; sh.col[0] = 0x7fffffff; }
       __syncthreads();
-      atomicMax(&count, best);
+      atomicMax(&sh.count, best);
       __syncthreads();
-      if (best == count) atomicMin(&cand_col[0], best_col);
+      if (best == sh.count) atomicMin(&sh.col[0], best_col);
       __syncthreads();
-      last_key = count;
-      last_col = cand_col[0];
+      last_key = sh.count;
+      last_col = sh.col[0];
       if (t == 0) put(place, last_key, last_col);
     }
   }
@@ -285,7 +402,7 @@ void token_logprob_kernel(LogprobArgs a) {
 
 // ---------------------------------------------------------------------------
 // Parts of rows merged: stats [n, 4, rows], alternatives [n, rows, top], sorted lists.  A wavefront per row with
-// alternatives (lane i holds the head of list i), a thread per row without.  Final values (logprob, entropy, lse), or,
+// alternatives or for few rows, a thread per row otherwise.  Final values (logprob, entropy, lse), or,
 // with out_stats, the statistics of the merged part.
 // ---------------------------------------------------------------------------
 struct LogprobCombineArgs {
@@ -303,22 +420,22 @@ struct LogprobCombineArgs {
 };
 static_assert(sizeof(LogprobCombineArgs) <= kCheapArgs, "");
 
-template <bool TOP>
-__global__ __launch_bounds__(TOP ? 64 : 256)
+template <bool WAVE>
+__global__ __launch_bounds__(WAVE ? 64 : 256)
 void token_logprob_combine_kernel(LogprobCombineArgs a) {
-  extern __shared__ __align__(16) unsigned char lists[];   // TOP: int64_t [n * top], then float [n * top]
-  const int row = TOP ? int(blockIdx.x) : int(blockIdx.x) * 256 + int(threadIdx.x);
+  extern __shared__ __align__(16) unsigned char lists[];   // tokens int64_t [n * top], then keys uint32_t [n * top]
+  const int row = WAVE ? int(blockIdx.x) : int(blockIdx.x) * 256 + int(threadIdx.x);
   if (row >= a.rows) return;
-  const int lane = TOP ? int(threadIdx.x) : 0;
+  const int lane = WAVE ? int(threadIdx.x) : 0;
   const int64_t R = a.rows;
   const int64_t token = a.tokens[row];
   const bool ignored = token == a.ignored_index;
-  LogprobTuple p = LogprobTuple::identity();
+  LogprobStats p = LogprobStats::identity();
   float picked = 0.f;
-  if constexpr (TOP) {
+  if constexpr (WAVE) {
     if (lane < a.n) {
       const float* s = a.stats + lane * 4 * R + row;
-      p = LogprobTuple{{s[0], s[R], s[2 * R]}};
+      p = LogprobStats{{s[0], s[R], s[2 * R]}};
       picked = s[3 * R];
     }
     p = wave_allreduce_tuple(p);
@@ -327,7 +444,7 @@ void token_logprob_combine_kernel(LogprobCombineArgs a) {
   } else {
     for (int k = 0; k < a.n; ++k) {
       const float* s = a.stats + k * 4 * R + row;
-      p = LogprobTuple::merge(p, LogprobTuple{{s[0], s[R], s[2 * R]}});
+      p = LogprobStats::merge(p, LogprobStats{{s[0], s[R], s[2 * R]}});
       picked += s[3 * R];
     }
   }
@@ -345,37 +462,97 @@ void token_logprob_combine_kernel(LogprobCombineArgs a) {
       if (a.lse) a.lse[row] = ignored ? 0.f : lse;
     }
   }
-  if constexpr (TOP) {
-    int64_t* lt = reinterpret_cast<int64_t*>(lists);
-    float* lv = reinterpret_cast<float*>(lt + a.n * a.top);
-    const int total = a.n * a.top;
-    for (int i = lane; i < total; i += kWave) {
-      const int64_t at = (int64_t(i / a.top) * R + row) * a.top + i % a.top;
-      lv[i] = a.in_value[at];
-      lt[i] = a.in_token[at];
-    }
-    __syncthreads();
+  if constexpr (WAVE) {
+    if (a.top == 0) return;   // uniform
+    const int total = a.n * a.top, each = (total + kWave - 1) / kWave;
+    int64_t* const lt = reinterpret_cast<int64_t*>(lists);
+    uint32_t* const lk = reinterpret_cast<uint32_t*>(lt + total);
     const bool none = !ignored && !a.out_stats && !(fabsf(lse) < __builtin_huge_valf());
     const float base = a.out_stats ? 0.f : lse;
-    int head = 0;
-    for (int place = 0; place < a.top; ++place) {
-      const bool have = !none && !ignored && lane < a.n && head < a.top && lt[lane * a.top + head] >= 0;
-      const float v = have ? lv[lane * a.top + head] : kNegInf;
-      const int64_t tok = have ? lt[lane * a.top + head] : 0x7fffffffffffffffLL;
-      const float best = wave_allreduce_tuple(MaxTuple{{v}}).v[0];
-      int64_t winner = have && v == best ? tok : 0x7fffffffffffffffLL;
-#pragma unroll
-      for (int s = 1; s < kWave; s *= 2) {
-        const int64_t o = __shfl_xor(winner, s, kWave);
-        winner = o < winner ? o : winner;
+    float* const value = a.top_value + int64_t(row) * a.top;
+    int64_t* const number = a.top_token + int64_t(row) * a.top;
+    auto put = [&](int place, uint32_t k, int64_t tok) {
+      value[place] = u2f(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)) - base;
+      number[place] = tok;
+    };
+    auto fill = [&](int found) {
+      if (lane < a.top && lane >= found) {
+        value[lane] = none ? __builtin_nanf("") : kNegInf;
+        number[lane] = -1;
       }
-      const bool found = winner != 0x7fffffffffffffffLL;   // uniform
-      if (have && tok == winner && v == best) ++head;
-      if (lane == 0) {
-        a.top_value[int64_t(row) * a.top + place] = found ? best - base : none ? __builtin_nanf("") : kNegInf;
-        a.top_token[int64_t(row) * a.top + place] = found ? winner : -1;
+    };
+    // a key of 0: no alternative
+    if (total <= kWave) {   // uniform: one a lane, each one's place among them
+      uint32_t k = 0;
+      int64_t tok = -1;
+      if (lane < total) {
+        const int64_t at = (int64_t(lane / a.top) * R + row) * a.top + lane % a.top;
+        tok = a.in_token[at];
+        k = none || ignored || tok < 0 ? 0 : order_key(a.in_value[at]);
+      }
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < total; ++j) {
+        const uint32_t kj = __builtin_amdgcn_readlane(int(k), j);
+        const int64_t tj = int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(tok >> 32), j))) << 32 |
+                                   uint32_t(__builtin_amdgcn_readlane(int(tok), j)));
+        place += (kj > k || (kj == k && tj < tok)) ? 1 : 0;
+      }
+      if (k != 0 && place < a.top) put(place, k, tok);
+      fill(__builtin_popcountll(__builtin_amdgcn_ballot_w64(k != 0)));
+      return;
+    }
+    constexpr int KEEP = 4;                 // keys that a lane keeps; the rest stay in LDS
+    uint32_t key[KEEP] = {};
+    for (int j = 0; j < each; ++j) {
+      const int i = j * kWave + lane;
+      if (i < total) {
+        const int64_t at = (int64_t(i / a.top) * R + row) * a.top + i % a.top;
+        const int64_t tok = a.in_token[at];
+        const uint32_t k = none || ignored || tok < 0 ? 0 : order_key(a.in_value[at]);
+        lt[i] = tok;
+        lk[i] = k;
+        static_for<KEEP>([&](auto q) { if (j == q) key[q] = k; });
       }
     }
+    __syncthreads();
+    // the k-th largest key by bisection, and how many reach it
+    uint32_t bound = 0;
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t at = bound | (1u << b);
+      int n = 0;
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[q] >= at));
+      for (int j = KEEP; j < each; ++j)
+        n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(j * kWave + lane < total && lk[j * kWave + lane] >= at));
+      if (n >= int(a.top)) bound = at;
+      if (n == int(a.top)) break;   // uniform
+    }
+    bound = max(bound, 1u);
+    // those, moved to the front of the list, and each one's place among them
+    int left = 0;
+    for (int j = 0; j < each; ++j) {
+      const int i = j * kWave + lane;
+      const uint32_t k = i < total ? lk[i] : 0;
+      const int64_t tok = i < total ? lt[i] : 0;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(k >= bound);
+      __syncthreads();   // (a place that is written was read in this round or before it)
+      if (k >= bound) {
+        const int to = left + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1));
+        lk[to] = k;
+        lt[to] = tok;
+      }
+      left += __builtin_popcountll(mask);
+      __syncthreads();
+    }
+    for (int i = lane; i < left; i += kWave) {
+      const uint32_t k = lk[i];
+      const int64_t tok = lt[i];
+      int place = 0;
+      for (int j = 0; j < left; ++j) place += (lk[j] > k || (lk[j] == k && lt[j] < tok)) ? 1 : 0;
+      if (place < a.top) put(place, k, tok);
+    }
+    fill(left);
   }
 }
 
@@ -389,16 +566,15 @@ struct LogprobBwdArgs {
   void* out;
   int64_t x_pitch, out_pitch, ignored_index, vocab_start;
   int cols, seg, segs;   // a workgroup takes `seg` columns of a row, a row has `segs` workgroups
+  uint16_t threads;
 };
 static_assert(sizeof(LogprobBwdArgs) <= kCheapArgs, "");
 
-constexpr int kBwdThreads = 256;
-
 template <typename T, bool RAGGED, bool ENTROPY>
-__global__ __launch_bounds__(kBwdThreads)
+__global__ __launch_bounds__(256)
 void token_logprob_bwd_kernel(LogprobBwdArgs a) {
-  constexpr int VEC = VecIO<T>::N;
-  const int t = int(threadIdx.x);
+  constexpr int VEC = VecIO<T>::N, U = RAGGED ? 2 : 1;
+  const int t = int(threadIdx.x), threads = a.threads;
   const uint32_t row = blockIdx.x / uint32_t(a.segs);
   const int first = int(blockIdx.x - row * uint32_t(a.segs)) * a.seg, cols = min(a.seg, a.cols - first);
   T* const outr = static_cast<T*>(a.out) + int64_t(row) * a.out_pitch + first;
@@ -410,12 +586,18 @@ void token_logprob_bwd_kernel(LogprobBwdArgs a) {
   if (token == a.ignored_index) {   // uniform
     const PartSpan<T, RAGGED> span(outr, cols, t);
     const float zero[VEC] = {};
-    for (int v = t; v < span.nvec; v += kBwdThreads) store(outr + span.column(v), zero);
+    for (int v = t; v < span.nvec; v += threads) store(outr + span.column(v), zero);
     if (RAGGED && span.edge >= 0) Cvt<T>::store(outr + span.edge, 0.f);
     return;
   }
   const T* const xr = static_cast<const T*>(a.logits) + int64_t(row) * a.x_pitch + first;
   const PartSpan<T, RAGGED> span(xr, cols, t);
+  u32x4 raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int v = u * threads + t;
+    if (v < span.nvec) raw[u] = span.load(v);
+  }
   const float lse = a.lse[row], g = a.g ? a.g[row] : 0.f;
   const float h = ENTROPY ? a.h[row] : 0.f;
   // dx = p (c0 - h log p) + g [j = token],  c0 = -g - h H
@@ -427,13 +609,17 @@ void token_logprob_bwd_kernel(LogprobBwdArgs a) {
     float o = ENTROPY ? p * fmaf(-h, fmaxf(lp, kFarBelow), c0) : p * c0;
     return col == hit ? o + g : o;
   };
-  for (int v = t; v < span.nvec; v += kBwdThreads) {
-    float f[VEC];
-    const int c = span.column(v);
-    VecIO<T>::unpack(span.load(v), f);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], c + j);
-    store(outr + c, f);
+  for (int u = 0; u < U; ++u) {
+    const int v = u * threads + t;
+    if (v < span.nvec) {
+      float f[VEC];
+      const int c = span.column(v);
+      VecIO<T>::unpack(raw[u], f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = grad(f[j], c + j);
+      store(outr + c, f);
+    }
   }
   if (RAGGED && span.edge >= 0) Cvt<T>::store(outr + span.edge, grad(Cvt<T>::load(xr + span.edge), span.edge));
 }
@@ -445,19 +631,22 @@ void token_logprob_bwd_kernel(LogprobBwdArgs a) {
 struct LogprobPlan {
   int splits, seg, threads;
 };
-static LogprobPlan plan_logprob(int64_t rows, int64_t cols, int vec) {
+static int pow2_at_least(int64_t n) {
+  int p = 64;
+  while (p < n && p < 512) p *= 2;
+  return p;
+}
+static LogprobPlan plan_logprob(int64_t rows, int64_t cols, int vec, int64_t top) {
   LogprobPlan p;
-  const int64_t nvec = (cols + vec - 1) / vec;
+  const int64_t nvec = (cols + vec - 1) / vec, cus = device_cu_count();
   p.splits = 1;
-  const int64_t want = 2 * int64_t(device_cu_count());
-  if (rows < want) {
-    const int64_t most = std::min<int64_t>(kMaxShards, (nvec + 1023) / 1024);
-    p.splits = int(std::max<int64_t>(1, std::min(most, want / std::max<int64_t>(rows, 1))));
-  }
+  const int64_t part = top ? 32768 : 2048;   // vectors
+  if (nvec >= 2 * part)
+    p.splits = int(std::max<int64_t>(1, std::min<int64_t>({nvec / part, cus / std::max<int64_t>(rows, 1), kMaxSplits})));
   const int64_t per = (nvec + p.splits - 1) / p.splits;
   p.seg = int(std::min<int64_t>(per * vec, 0x7fffffff));
   p.splits = int((cols + p.seg - 1) / p.seg);
-  p.threads = int(std::min<int64_t>(1024, std::max<int64_t>(64, ((per + 3) / 4 + 63) / 64 * 64)));
+  p.threads = rows * p.splits <= cus ? std::max(128, pow2_at_least(per / 4)) : std::min(256, std::max(top ? 128 : 64, pow2_at_least(per / 32)));
   return p;
 }
 static size_t logprob_workspace(const LogprobPlan& p, int64_t rows, int top) {
@@ -465,7 +654,7 @@ static size_t logprob_workspace(const LogprobPlan& p, int64_t rows, int top) {
 }
 
 static int launch_combine(const LogprobCombineArgs& a, hipStream_t s) {
-  if (a.top) {
+  if (a.top || a.rows <= 1024) {
     HK_LAUNCH((token_logprob_combine_kernel<true>), dim3(unsigned(a.rows)), dim3(64), size_t(a.n) * a.top * 12, s, a);
   } else {
     HK_LAUNCH((token_logprob_combine_kernel<false>), dim3(unsigned((a.rows + 255) / 256)), dim3(256), 0, s, a);
@@ -490,7 +679,7 @@ static int logprob_forward(const char* name, int dtype, const void* logits, int6
   HK_REQUIRE(top == 0 || (top_value && top_token), HK_ERR_INVALID, "%s: null alternatives", name);
   HK_REQUIRE(pitch >= cols, HK_ERR_INVALID, "%s: row pitch %lld below %lld columns", name, (long long)pitch, (long long)cols);
   const int vec = int(16 / dtype_size(dtype));
-  const LogprobPlan p = plan_logprob(rows, cols, vec);
+  const LogprobPlan p = plan_logprob(rows, cols, vec, top);
   const size_t need = logprob_workspace(p, rows, int(top));
   HK_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), HK_ERR_WORKSPACE,
              "%s: workspace of %zu bytes needed, %zu given", name, need, workspace_bytes);
@@ -527,8 +716,11 @@ static int logprob_forward(const char* name, int dtype, const void* logits, int6
     if (top && r) { b.top_value = a.top_value + r * top; b.top_token = a.top_token + r * top; }
     const dim3 grid = mode1 ? dim3(unsigned(p.splits), unsigned(n)) : dim3(unsigned(n));
     const dim3 block{unsigned(p.threads)};
+    // (the slots that rows of this length use)
+    const int64_t rounds = (p.seg / vec + p.threads * 32 / vec - 1) / (p.threads * 32 / vec) + 1;
+    const size_t lds = top ? size_t(std::min<int64_t>(kMaxSlots, rounds)) * p.threads * sizeof(float) : 0;
     profile_before(s);
-#define HK_LP(T, RAGGED, MODE, TOP) HK_LAUNCH((token_logprob_kernel<T, RAGGED, MODE, TOP>), grid, block, 0, s, b)
+#define HK_LP(T, RAGGED, MODE, TOP) HK_LAUNCH((token_logprob_kernel<T, RAGGED, MODE, TOP>), grid, block, lds, s, b)
 #define HK_LP_TOP(T, RAGGED, MODE) do { if (top) HK_LP(T, RAGGED, MODE, true); else HK_LP(T, RAGGED, MODE, false); } while (0)
 #define HK_LP_MODE(T, RAGGED) do { if (mode1) HK_LP_TOP(T, RAGGED, 1); else HK_LP_TOP(T, RAGGED, 0); } while (0)
 #define HK_LP_TYPE(T) do { if (ragged) HK_LP_MODE(T, true); else HK_LP_MODE(T, false); } while (0)
@@ -562,7 +754,7 @@ int hk_token_logprob_workspace_bytes(int dtype, int64_t rows, int64_t cols, int6
   HK_REQUIRE(is_row_dtype(dtype), HK_ERR_UNSUPPORTED, "hk_token_logprob_workspace_bytes: not implemented for dtype %d", dtype);
   HK_REQUIRE(bytes && rows >= 0 && cols >= 1 && top >= 0 && top <= kMaxTop && rows <= 0x7fffffffLL && cols <= 0x7ffffff0LL,
              HK_ERR_INVALID, "hk_token_logprob_workspace_bytes: bad argument");
-  *bytes = rows == 0 ? 0 : logprob_workspace(plan_logprob(rows, cols, int(16 / dtype_size(dtype))), rows, int(top));
+  *bytes = rows == 0 ? 0 : logprob_workspace(plan_logprob(rows, cols, int(16 / dtype_size(dtype)), top), rows, int(top));
   return HK_OK;
 }
 
@@ -624,9 +816,9 @@ int hk_token_logprob_bwd(int dtype, const void* logits, int64_t logits_pitch, co
   a.logits = logits; a.tokens = tokens; a.lse = lse; a.entropy = entropy; a.g = grad_logprob; a.h = grad_entropy; a.out = dlogits;
   a.x_pitch = logits_pitch; a.out_pitch = dlogits_pitch; a.ignored_index = ignored_index; a.vocab_start = vocab_start;
   a.cols = int(cols);
-  const int64_t nvec = (cols + vec - 1) / vec;
-  const int64_t parts = (nvec + 4 * kBwdThreads - 1) / (4 * kBwdThreads), per = (nvec + parts - 1) / parts;
-  a.seg = int(std::min<int64_t>(per * vec, 0x7fffffff));
+  const int threads = ragged ? 256 : dtype == HK_FLOAT32 ? 64 : 128;
+  a.threads = uint16_t(threads);
+  a.seg = (ragged ? 2 : 1) * threads * vec;
   a.segs = int((cols + a.seg - 1) / a.seg);
   hipStream_t s = as_hip(stream);
   const int64_t at_once = std::max<int64_t>(1, 0x7fffffffLL / a.segs);   // workgroups of a launch fit 31 bits
@@ -640,7 +832,7 @@ int hk_token_logprob_bwd(int dtype, const void* logits, int64_t logits_pitch, co
     if (b.entropy) b.entropy += r;
     if (b.g) b.g += r;
     if (b.h) b.h += r;
-    const dim3 grid{unsigned(n * a.segs)}, block{unsigned(kBwdThreads)};
+    const dim3 grid{unsigned(n * a.segs)}, block{unsigned(threads)};
     profile_before(s);
 #define HK_LP(T, RAGGED) \
   do { if (grad_entropy) HK_LAUNCH((token_logprob_bwd_kernel<T, RAGGED, true>), grid, block, 0, s, b); \

@@ -27,7 +27,7 @@
 
 namespace {
 
-PyObject *s_data_ptr, *s_is_contiguous, *s_shape, *s_stride, *s_dtype, *s_is_cuda, *s_get_device, *s_value;
+PyObject *s_numel, *s_data_ptr, *s_is_contiguous, *s_shape, *s_stride, *s_dtype, *s_is_cuda, *s_get_device, *s_value;
 PyObject* g_dtype_codes;      // {torch dtype: code}
 PyObject* g_current_stream;   // () -> address of torch's current stream (initialises the device if need be)
 PyObject *g_get_device, *g_raw_stream;   // torch's own two steps of the same, once the device is initialised
@@ -338,6 +338,105 @@ PyObject* rows_cols(PyObject*, PyObject* t) {
   return Py_BuildValue("LL", (long long)(cols == 0 ? 0 : rows), (long long)cols);
 }
 
+// What the newer operators' harness asks of its operands before a call.  Each answers None / False where something does not
+// fit; the harness then looks for what it was and says so.
+// rows of a tensor with a unit-stride last dimension: (rows, cols, pitch); false where it is neither dense nor 2-D
+bool rows_of(PyObject* t, int64_t* rows, int64_t* cols, int64_t* pitch) {
+  PyObject* shape = PyObject_GetAttr(t, s_shape);
+  if (shape == nullptr) return false;
+  *rows = *cols = 1;
+  int64_t last_but_one = 1;
+  const Py_ssize_t n = each_i64(shape, [&](Py_ssize_t, int64_t v) { *rows *= *cols; last_but_one = *cols; *cols = v; });
+  Py_DECREF(shape);
+  if (n < 1) return false;
+  *pitch = *cols;
+  PyObject* c = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+  if (c == nullptr) return false;
+  const int dense = PyObject_IsTrue(c);
+  Py_DECREF(c);
+  if (dense != 0) return dense > 0;
+  if (n != 2) return false;
+  PyObject* stride = PyObject_CallMethodNoArgs(t, s_stride);
+  if (stride == nullptr) return false;
+  int64_t st[2] = {0, 0};
+  const Py_ssize_t k = each_i64(stride, [&](Py_ssize_t i, int64_t v) { if (i < 2) st[i] = v; });
+  Py_DECREF(stride);
+  if (k != 2 || (*cols > 1 && st[1] != 1)) return false;
+  if (last_but_one > 1) *pitch = st[0];
+  return true;
+}
+int64_t device_of(PyObject* t) {
+  PyObject* d = PyObject_CallMethodNoArgs(t, s_get_device);
+  if (d == nullptr) return -2;
+  int64_t v = -2;
+  to_i64(d, &v);
+  Py_DECREF(d);
+  return v;
+}
+PyObject* answer_none() {   // an error on the way is the harness's to find again
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+// row_operand(t): (rows, cols, pitch, dtype code, device) of a [.., cols] operand on the current device, or None
+PyObject* row_operand(PyObject*, PyObject* t) {
+  int64_t rows, cols, pitch;
+  if (!rows_of(t, &rows, &cols, &pitch)) return answer_none();
+  const int code = dtype_code_of(t);
+  if (code < 0) return answer_none();
+  const int64_t dev = device_of(t);
+  if (dev < 0 || g_get_device == Py_None) return answer_none();
+  PyObject* cur = PyObject_CallNoArgs(g_get_device);
+  int64_t current = -1;
+  const bool ok = cur != nullptr && to_i64(cur, &current) && current == dev;
+  Py_XDECREF(cur);
+  if (!ok) return answer_none();
+  return Py_BuildValue("LLLiL", (long long)(cols == 0 ? 0 : rows), (long long)cols, (long long)pitch, code, (long long)dev);
+}
+// row_pitches(rows, cols, code, device, a, b, ...): the pitches of operands of that shape, type and device (of None: cols)
+PyObject* row_pitches(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  int64_t rows, cols, code, dev;
+  if (n < 4 || !to_i64(args[0], &rows) || !to_i64(args[1], &cols) || !to_i64(args[2], &code) || !to_i64(args[3], &dev)) return answer_none();
+  PyObject* out = PyTuple_New(n - 4);
+  if (out == nullptr) return nullptr;
+  for (Py_ssize_t i = 4; i < n; ++i) {
+    int64_t r = rows, c = cols, p = cols;
+    if (args[i] != Py_None &&
+        (!rows_of(args[i], &r, &c, &p) || (c == 0 ? 0 : r) != rows || c != cols || dtype_code_of(args[i]) != code || device_of(args[i]) != dev)) {
+      Py_DECREF(out);
+      return answer_none();
+    }
+    PyObject* v = PyLong_FromLongLong(p);
+    if (v == nullptr) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i - 4, v);
+  }
+  return out;
+}
+// values(count, code, device, a, b, ...): whether every operand is None or dense with `count` values of that type there
+PyObject* values(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  int64_t count, code, dev;
+  if (n < 3 || !to_i64(args[0], &count) || !to_i64(args[1], &code) || !to_i64(args[2], &dev)) return answer_none();
+  for (Py_ssize_t i = 3; i < n; ++i) {
+    if (args[i] == Py_None) continue;
+    PyObject* numel = PyObject_CallMethodNoArgs(args[i], s_numel);
+    int64_t have = -1;
+    bool ok = numel != nullptr && to_i64(numel, &have) && have == count && dtype_code_of(args[i]) == code && device_of(args[i]) == dev;
+    Py_XDECREF(numel);
+    if (ok) {
+      PyObject* c = PyObject_CallMethodNoArgs(args[i], s_is_contiguous);
+      ok = c != nullptr && PyObject_IsTrue(c) == 1;
+      Py_XDECREF(c);
+    }
+    if (!ok) {
+      PyErr_Clear();
+      Py_RETURN_FALSE;
+    }
+  }
+  Py_RETURN_TRUE;
+}
+
 PyObject* setup(PyObject*, PyObject* args) {
   return PyArg_ParseTuple(args, "OOOO", &g_dtype_codes, &g_current_stream, &g_get_device, &g_raw_stream)
              ? (Py_INCREF(g_dtype_codes), Py_INCREF(g_current_stream), Py_INCREF(g_get_device), Py_INCREF(g_raw_stream),
@@ -351,6 +450,9 @@ PyMethodDef methods[] = {
     {"setup", setup, METH_VARARGS, nullptr},
     {"dense", (PyCFunction)(void (*)())dense, METH_FASTCALL, nullptr},
     {"rows_cols", rows_cols, METH_O, nullptr},
+    {"row_operand", row_operand, METH_O, nullptr},
+    {"row_pitches", (PyCFunction)(void (*)())row_pitches, METH_FASTCALL, nullptr},
+    {"values", (PyCFunction)(void (*)())values, METH_FASTCALL, nullptr},
 #ifndef HT_CALL
     ENTRY(dropout_fwd_ex), ENTRY(dropout_bwd_ex), ENTRY(hk_batch_norm_bwd), ENTRY(hk_batch_norm_fwd),
     ENTRY(hk_binary_const), ENTRY(hk_dropout_add_ln_bwd_pitched), ENTRY(hk_dropout_add_ln_fwd_pitched),
@@ -390,7 +492,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, MODULE_NAME, nullptr, -1, methods, 
 
 PyMODINIT_FUNC MODULE_INIT(void) {
   const std::pair<PyObject**, const char*> names[] = {
-      {&s_data_ptr, "data_ptr"}, {&s_is_contiguous, "is_contiguous"}, {&s_shape, "shape"}, {&s_stride, "stride"},
+      {&s_numel, "numel"}, {&s_data_ptr, "data_ptr"}, {&s_is_contiguous, "is_contiguous"}, {&s_shape, "shape"}, {&s_stride, "stride"},
       {&s_dtype, "dtype"}, {&s_is_cuda, "is_cuda"}, {&s_get_device, "get_device"}, {&s_value, "value"}};
   for (const auto& n : names)
     if ((*n.first = PyUnicode_InternFromString(n.second)) == nullptr) return nullptr;
