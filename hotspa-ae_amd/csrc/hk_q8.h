@@ -12,52 +12,66 @@ namespace hk {
 constexpr int kQ8Block = 32;
 inline int64_t q8_blocks(int64_t cols) { return (cols + kQ8Block - 1) / kQ8Block; }
 
-// A row's columns [c, c + N) of R as floats, c a multiple of N; 0 past the row's end.  TAIL: the row may end inside a
-// vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector inside
-// the row and none sits in a branch.  raw() is the load, floats() what comes of it.
+// A row's columns [c, c + N) of R as floats, c a multiple of N; 0 past the row's end: one load of 16 bytes, or of 8 where a
+// 16-bit operand goes along with an fp32 one (neighbouring lanes then read neighbouring memory in both: a residual stream in
+// fp32 beside bf16 rows, read as two 16-byte loads 32 bytes apart, 405 us instead of 270 for 32768 x 4096).  TAIL: the row may end before
+// or inside a vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector
+// inside the row and none sits in a branch; without it every vector lies inside.  raw is the load, floats() what comes of it.
+typedef u32x2 u32x2_on2 __attribute__((aligned(2)));
 template <typename R, int N, bool TAIL>
 struct RowVec {
-  static constexpr int M = VecIO<R>::N, K = N / M;   // elements and number of 16-byte loads
-  static_assert(N % M == 0, "whole loads");
-  u32x4 raw[K];
+  static constexpr int kWords = N * int(sizeof(R)) / 4;
+  static_assert(kWords == 4 || kWords == 2, "one load of 16 or 8 bytes");
+  u32x4 raw;
   // row: any element boundary; one of cols elements, cols >= 1
-  __device__ __forceinline__ void load(const R* row, int c, int cols, bool keep) {
-    if (TAIL && cols < M) {   // uniform: a row shorter than a load
-#pragma unroll
-      for (int k = 0; k < K; ++k) raw[k] = u32x4{0, 0, 0, 0};
+  template <bool KEEP = false>   // KEEP: read by many workgroups
+  __device__ __forceinline__ void load(const R* row, int c, int cols) {
+    if (TAIL && cols < N) {   // uniform: a row shorter than a load
+      float f[8] = {};
       if (c == 0) {
-        float f[M] = {};
 #pragma unroll
-        for (int j = 0; j < M; ++j)
+        for (int j = 0; j < N; ++j)
           if (j < cols) f[j] = Cvt<R>::load(row + j);
-        raw[0] = VecIO<R>::pack(f);
       }
+      raw = VecIO<R>::pack(f);
       return;
     }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int at = c + k * M, from = min(at, cols - M);
-      raw[k] = keep ? ld16_any_keep<R>(row + from) : ld16_any<R>(row + from);
+    // (a scalar base and 32 bits of offset)
+    const R* p = reinterpret_cast<const R*>(reinterpret_cast<const char*>(row) + uint32_t(TAIL ? min(c, cols - N) : c) * uint32_t(sizeof(R)));
+    if constexpr (kWords == 4) {
+      if constexpr (KEEP) raw = ld16_any_keep<R>(p);
+      else raw = ld16_any<R>(p);
+    } else {
+      u32x2 w;
+      if constexpr (KEEP) w = *reinterpret_cast<const u32x2_on2*>(p);
+      else w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_on2*>(p));
+      raw = u32x4{w.x, w.y, 0, 0};
     }
   }
   __device__ __forceinline__ void floats(float* f, int c, int cols) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      u32x4 r = raw[k];
-      const int at = c + k * M;
-      if constexpr (TAIL) {
-        if (cols >= M) {   // uniform
-          const int bits = (at - min(at, cols - M)) * int(sizeof(R)) * 8;
-          const uint64_t lo = uint64_t(r.y) << 32 | r.x, hi = uint64_t(r.w) << 32 | r.z;
-          const uint64_t in = bits & 63 ? hi << (64 - (bits & 63)) : 0;
+    u32x4 r = raw;
+    if constexpr (TAIL) {
+      if (cols >= N) {   // uniform
+        const int bits = (c - min(c, cols - N)) * int(sizeof(R)) * 8;
+        const uint64_t lo = uint64_t(r.y) << 32 | r.x;
+        if constexpr (kWords == 2) {
+          const uint64_t l = bits < 64 ? lo >> (bits & 63) : 0;
+          r = u32x4{uint32_t(l), uint32_t(l >> 32), 0, 0};
+        } else {
+          const uint64_t hi = uint64_t(r.w) << 32 | r.z, in = bits & 63 ? hi << (64 - (bits & 63)) : 0;
           uint64_t l = bits >= 64 ? hi >> (bits & 63) : (lo >> (bits & 63)) | in, h = bits >= 64 ? 0 : hi >> (bits & 63);
           if (bits >= 128) l = 0;
           r = u32x4{uint32_t(l), uint32_t(l >> 32), uint32_t(h), uint32_t(h >> 32)};
         }
-      } else if (at >= cols) {
-        r = u32x4{0, 0, 0, 0};
       }
-      VecIO<R>::unpack(r, f + k * M);
+    }
+    if constexpr (kWords == 4) {
+      VecIO<R>::unpack(r, f);
+    } else {
+      float e[8];
+      VecIO<R>::unpack(r, e);
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = e[j];
     }
   }
 };
@@ -65,25 +79,25 @@ struct RowVec {
 // stores N floats as R at columns [c, c + N) of a row, those inside it
 template <typename R, int N, bool TAIL>
 __device__ __forceinline__ void store_row_floats(R* row, int c, int cols, const float* f) {
-  constexpr int M = VecIO<R>::N;
+  constexpr int kWords = N * int(sizeof(R)) / 4;
+  float e[8];
 #pragma unroll
-  for (int k = 0; k < N / M; ++k) {
-    const int at = c + k * M, left = cols - at;
-    const u32x4 r = VecIO<R>::pack(f + k * M);
-    if (left >= M) {
-      st16_any(row + at, r);
-    } else if (TAIL && left > 0) {
-      typedef uint32_t word __attribute__((aligned(2)));
-      R* p = row + at;
-      uint32_t w[4] = {r.x, r.y, r.z, r.w};
-      int words = left * int(sizeof(R)) / 4;
+  for (int j = 0; j < 8; ++j) e[j] = j < N ? f[j] : 0.f;
+  const u32x4 r = VecIO<R>::pack(e);
+  const int left = cols - c;
+  R* p = reinterpret_cast<R*>(reinterpret_cast<char*>(row) + uint32_t(c) * uint32_t(sizeof(R)));
+  if (!TAIL || left >= N) {
+    if constexpr (kWords == 4) st16_any(p, r);
+    else __builtin_nontemporal_store(u32x2{r.x, r.y}, reinterpret_cast<u32x2_on2*>(p));
+  } else if (left > 0) {
+    typedef uint32_t word __attribute__((aligned(2)));
+    const int words = left * int(sizeof(R)) / 4;
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (i < words) reinterpret_cast<word*>(p)[i] = w[i];
-      if (sizeof(R) == 2 && (left & 1)) {
-        const uint32_t last = words == 0 ? w[0] : words == 1 ? w[1] : words == 2 ? w[2] : w[3];
-        reinterpret_cast<uint16_t*>(p)[left - 1] = uint16_t(last);
-      }
+    for (int i = 0; i < kWords - 1; ++i)
+      if (i < words) reinterpret_cast<word*>(p)[i] = r[i];
+    if (sizeof(R) == 2 && (left & 1)) {
+      const uint32_t last = words == 0 ? r.x : words == 1 ? r.y : words == 2 ? r.z : r.w;
+      reinterpret_cast<uint16_t*>(p)[left - 1] = uint16_t(last);
     }
   }
 }
@@ -116,10 +130,10 @@ __device__ __forceinline__ float q8_step(uint32_t exponent) {
   const uint32_t bits = exponent >= 7 ? (exponent - 6) << 23 : 1u << (exponent + 16);
   return u2f(exponent == 255 ? 0x7fc00000u : bits);
 }
-// the values of 4 bytes
-__device__ __forceinline__ void q8_decode4(uint32_t bytes, float step, float* f) {
+// the whole numbers of 4 bytes
+__device__ __forceinline__ void q8_numbers4(uint32_t bytes, float* f) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) f[j] = float(int8_t(bytes >> (8 * j))) * step;
+  for (int j = 0; j < 4; ++j) f[j] = float(int8_t(bytes >> (8 * j)));
 }
 
 // the words of N elements, N = 4 or 8
@@ -129,18 +143,15 @@ template <> struct Q8Words<8> {
   static __device__ __forceinline__ type encode(const float* f, float factor) {
     return u32x2{q8_encode4(f, factor), q8_encode4(f + 4, factor)};
   }
-  static __device__ __forceinline__ void decode(type w, uint32_t exponent, float* f) {
-    const float step = q8_step(exponent);
-    q8_decode4(w.x, step, f);
-    q8_decode4(w.y, step, f + 4);
+  static __device__ __forceinline__ void numbers(type w, float* f) {
+    q8_numbers4(w.x, f);
+    q8_numbers4(w.y, f + 4);
   }
 };
 template <> struct Q8Words<4> {
   typedef uint32_t type;
   static __device__ __forceinline__ type encode(const float* f, float factor) { return q8_encode4(f, factor); }
-  static __device__ __forceinline__ void decode(type w, uint32_t exponent, float* f) {
-    q8_decode4(w, q8_step(exponent), f);
-  }
+  static __device__ __forceinline__ void numbers(type w, float* f) { q8_numbers4(w, f); }
 };
 
 // ---------------------------------------------------------------------------
@@ -168,9 +179,14 @@ struct Q8BwdArgs {
   float inv_cols;
   int rows, cols, blocks, grid;
   uint16_t threads;
+  bool few;                 // part_dgamma / part_dbeta are then dgamma / dbeta themselves
 };
 
 constexpr int kQ8MaxCols = 32768;
+
+// columns of a lane's vector: see RowVec
+template <typename T, typename RT>
+constexpr int q8_vec() { return sizeof(T) == 2 && sizeof(RT) == 2 ? 8 : 4; }
 
 // Lanes that hold a row and vectors per lane: lanes of a wavefront (8, 16, 32, 64) or, above 64, a workgroup's threads.
 struct Q8Shape {
@@ -179,7 +195,7 @@ struct Q8Shape {
 Q8Shape q8_fwd_shape(int64_t cols, int vec);
 Q8Shape q8_bwd_shape(int64_t cols, int vec);
 // workgroups of the backward kernel
-int q8_bwd_grid(int64_t rows, const Q8Shape& shape);
+int q8_bwd_grid(int64_t rows, const Q8Shape& shape, bool extra);
 
 template <typename T> int q8_norm_fwd_typed(const Q8FwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, hipStream_t s);
 template <typename T> int q8_norm_bwd_typed(const Q8BwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, void* dgamma,

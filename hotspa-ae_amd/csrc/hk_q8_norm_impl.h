@@ -32,7 +32,7 @@ struct Q8Group {
 template <typename T, typename RT, int NV, int LPR, bool HAS_RES, bool IS_RMS, bool TAIL>
 __global__ __launch_bounds__(LPR ? 256 : 1024)
 void q8_norm_fwd_kernel(Q8FwdArgs a) {
-  constexpr int VEC = VecIO<T>::N, LPB = kQ8Block / VEC;
+  constexpr int VEC = q8_vec<T, RT>(), LPB = kQ8Block / VEC;
   using Group = Q8Group<LPR>;
   using Words = Q8Words<VEC>;
   __shared__ float red[2][kMaxWaves * 2];
@@ -50,8 +50,8 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     const RT* rr = HAS_RES ? static_cast<const RT*>(a.residual) + row * a.res_pitch : nullptr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      x[i].load(xr, column(i), cols, false);
-      if constexpr (HAS_RES) r[i].load(rr, column(i), cols, false);
+      x[i].load(xr, column(i), cols);
+      if constexpr (HAS_RES) r[i].load(rr, column(i), cols);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -97,7 +97,7 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
       const int left = cols - column(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float d = j < left ? v[i][j] - mu : 0.f;
+        const float d = !TAIL || j < left ? v[i][j] - mu : 0.f;
         s.v[0] = fmaf(d, d, s.v[0]);
       }
     }
@@ -116,7 +116,7 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     const uint32_t e = q8_exponent<VEC>(v[i]);
     const typename Words::type w = Words::encode(v[i], q8_factor(e));
     const int c = column(i);
-    if (c < a.blocks * kQ8Block) {
+    if (!TAIL || c < a.blocks * kQ8Block) {
       *reinterpret_cast<typename Words::type*>(qr + c) = w;
       if (t % LPB == 0) sr[c / kQ8Block] = uint8_t(e);
     }
@@ -130,8 +130,8 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     const int c = column(i);
     float g[VEC], b[VEC], f[VEC];
     RowVec<T, VEC, TAIL> p;
-    if (gp) { p.load(gp, c, cols, true); p.floats(g, c, cols); }   // uniform
-    if (bp) { p.load(bp, c, cols, true); p.floats(b, c, cols); }
+    if (gp) { p.template load<true>(gp, c, cols); p.floats(g, c, cols); }   // uniform
+    if (bp) { p.template load<true>(bp, c, cols); p.floats(b, c, cols); }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const float n = rs * (v[i][j] - shift);
@@ -142,12 +142,18 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
 }
 
 // A persistent grid walks the rows; a thread keeps its columns' sums of dz x^ and dz, and the workgroup leaves one fp32
-// partial row of each.  The next row's loads are under way while a row is worked on.
+// partial row of each.  PF rows' loads are under way while a row is worked on (a ring of register slots; no load sits in a
+// branch).  EXTRA: an upstream gradient comes in.
 // MAXT: the most threads of a workgroup; above 512 the register budget is half of what the widest rows would take.
-template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, bool TAIL>
+#ifndef Q8_PF
+#define Q8_PF 1
+#endif
+template <int NV, bool EXTRA, int MAXT>
+constexpr int q8_prefetch() { return MAXT > 512 ? 1 : NV <= 2 ? Q8_PF : NV == 4 ? (Q8_PF > 1 ? 2 : 1) : 1; }
+template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, bool TAIL, int PF = q8_prefetch<NV, EXTRA, MAXT>()>
 __global__ __launch_bounds__(MAXT)
 void q8_norm_bwd_kernel(Q8BwdArgs a) {
-  constexpr int VEC = VecIO<T>::N, NE = NV * VEC;
+  constexpr int VEC = q8_vec<T, RT>(), NE = NV * VEC;
   using Group = Q8Group<LPR>;
   using Words = Q8Words<VEC>;
   constexpr int KS = IS_RMS ? 1 : 2;
@@ -157,18 +163,24 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   const int cols = a.cols, pitch = a.blocks * kQ8Block;
   auto column = [&](int i) { return (i * tpr + t) * VEC; };
 
-  float gm[NE], dg[NE];
+  float dg[NE];
   [[maybe_unused]] float db[IS_RMS ? 1 : NE];
   const T* gp = static_cast<const T*>(a.gamma);
+  // gamma as fp32, packed where that is more registers than there are
+  constexpr bool kPacked = NE > 16 && sizeof(T) == 2;
+  RowVec<T, VEC, TAIL> gm[NV];
+  [[maybe_unused]] float gf[kPacked ? 1 : NE];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (gp) {   // uniform
+      gm[i].template load<true>(gp, column(i), cols);
+    } else {
+      float one[8];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) gm[i * VEC + j] = 1.f;
-    if (gp) {
-      RowVec<T, VEC, TAIL> p;
-      p.load(gp, column(i), cols, true);
-      p.floats(&gm[i * VEC], column(i), cols);
+      for (int j = 0; j < 8; ++j) one[j] = 1.f;
+      gm[i].raw = VecIO<T>::pack(one);
     }
+    if constexpr (!kPacked) gm[i].floats(&gf[i * VEC], gp ? column(i) : 0, gp ? cols : VEC);   // (ones need no moving)
   }
 #pragma unroll
   for (int e = 0; e < NE; ++e) {
@@ -181,87 +193,102 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
     typename Words::type q[NV];
     uint8_t e[NV];
     float mu, rs;
-  } next;
+  } next[PF];
   const int64_t last = a.rows - 1;
-  auto issue = [&](int64_t r) {
+  auto issue = [&](auto slot, int64_t r) {   // a row past the end reads the last one, which is then not used
+    Slot& to = next[decltype(slot)::value];
     const int64_t rc = r < last ? r : last;
-    next.rs = a.rs[rc];
-    if constexpr (!IS_RMS) next.mu = a.mu[rc];
+    to.rs = a.rs[rc];
+    if constexpr (!IS_RMS) to.mu = a.mu[rc];
     const T* dr = static_cast<const T*>(a.dz) + rc * a.dz_pitch;
     const int8_t* qr = a.q + rc * int64_t(pitch);
     const uint8_t* sr = a.scale + rc * int64_t(a.blocks);
+    const RT* ur = EXTRA ? static_cast<const RT*>(a.dx_in) + rc * a.dxin_pitch : nullptr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = min(column(i), pitch - VEC);
-      next.dz[i].load(dr, column(i), cols, false);
-      next.q[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Words::type*>(qr + c));
-      next.e[i] = sr[c / kQ8Block];
-      if constexpr (EXTRA) {
-        if (a.dx_in) next.up[i].load(static_cast<const RT*>(a.dx_in) + rc * a.dxin_pitch, column(i), cols, false);
-      }
+      const uint32_t c = uint32_t(TAIL ? min(column(i), pitch - VEC) : column(i));
+      to.dz[i].load(dr, column(i), cols);
+      to.q[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Words::type*>(qr + c));
+      to.e[i] = sr[c / kQ8Block];
+      if constexpr (EXTRA) to.up[i].load(ur, column(i), cols);
     }
   };
   const int64_t stride = int64_t(a.grid) * Group::kRows;
   int64_t base = int64_t(blockIdx.x) * Group::kRows;
   int parity = 0;
-  issue(base + group);
-#pragma nounroll
-  for (; base < a.rows; base += stride) {   // uniform over the workgroup
-    const int64_t row = base + group;
-    const bool valid = LPR == 0 || row < a.rows;
+  static_for<PF>([&](auto slot) { issue(slot, base + group + decltype(slot)::value * stride); });
+  // GUARDED: the slot's row may not exist (the tail)
+  auto step = [&](auto slot, auto guarded) {
+    constexpr bool GUARD = decltype(guarded)::value;
+    Slot& in = next[decltype(slot)::value];
+    const int64_t row = base + group + decltype(slot)::value * stride;
+    const bool valid = !GUARD || row < a.rows;
     float x[NE], u[NE];
-    [[maybe_unused]] float up[EXTRA ? NE : 1];
-    const float rs = next.rs;
-    const float mu = IS_RMS ? 0.f : next.mu;
+    [[maybe_unused]] RowVec<RT, VEC, TAIL> up[EXTRA ? NV : 1];   // (packed until it is added)
+    const float rs = in.rs;
+    [[maybe_unused]] const float shift = IS_RMS ? 0.f : -rs * in.mu;
+    float step_of[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column(i);
-      next.dz[i].floats(&u[i * VEC], c, cols);
-      Words::decode(next.q[i], next.e[i], &x[i * VEC]);
-      if constexpr (EXTRA) {
-        if (a.dx_in) next.up[i].floats(&up[i * VEC], c, cols);
-      }
+      in.dz[i].floats(&u[i * VEC], column(i), cols);
+      Words::numbers(in.q[i], &x[i * VEC]);
+      step_of[i] = rs * q8_step(in.e[i]);   // (a power of two: exact)
+      if constexpr (EXTRA) up[i] = in.up[i];
     }
-    issue(row + stride);
+    issue(slot, row + PF * stride);
     SumTuple<KS> s = SumTuple<KS>::identity();
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const float dz = valid ? u[e] : 0.f;           // 0 past the row's end
-      // (nothing past the row's end, where another column's value or a NaN block's may stand)
-      x[e] = column(e / VEC) + (TAIL ? e % VEC : 0) < cols ? rs * (x[e] - mu) : 0.f;
-      dg[e] = fmaf(dz, x[e], dg[e]);
-      if constexpr (!IS_RMS) db[e] += dz;
-      u[e] = dz * gm[e];
-      s.v[KS - 1] = fmaf(u[e], x[e], s.v[KS - 1]);
-      if constexpr (!IS_RMS) s.v[0] += u[e];
+    for (int i = 0; i < NV; ++i) {
+      float g[VEC];
+      if constexpr (kPacked) gm[i].floats(g, gp ? column(i) : 0, gp ? cols : VEC);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) if constexpr (!kPacked) g[j] = gf[i * VEC + j];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int e = i * VEC + j;
+        const float dz = valid ? u[e] : 0.f;           // 0 past the row's end
+        x[e] = IS_RMS ? x[e] * step_of[i] : fmaf(x[e], step_of[i], shift);
+        // (nothing past the row's end, where another column's value or a NaN block's may stand)
+        if constexpr (TAIL) x[e] = column(i) + j < cols ? x[e] : 0.f;
+        dg[e] = fmaf(dz, x[e], dg[e]);
+        if constexpr (!IS_RMS) db[e] += dz;
+        u[e] = dz * g[j];
+        s.v[KS - 1] = fmaf(u[e], x[e], s.v[KS - 1]);
+        if constexpr (!IS_RMS) s.v[0] += u[e];
+      }
     }
     s = Group::allreduce(s, red[parity], tpr);
     parity ^= 1;
     if (valid) {
-      const float k1 = IS_RMS ? 0.f : s.v[0] * a.inv_cols, k2 = s.v[KS - 1] * a.inv_cols;
+      const float k1 = IS_RMS ? 0.f : -rs * (s.v[0] * a.inv_cols), k2 = -rs * (s.v[KS - 1] * a.inv_cols);
       T* dxr = static_cast<T*>(a.dx0) + row * a.dx_pitch;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float o[VEC];
+        [[maybe_unused]] float add[VEC];
+        if constexpr (EXTRA) up[i].floats(add, column(i), cols);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int e = i * VEC + j;
-          o[j] = rs * fmaf(-x[e], k2, u[e] - k1);
-          if constexpr (EXTRA) {
-            if (a.dx_in) o[j] += up[e];
-          }
+          o[j] = fmaf(x[e], k2, IS_RMS ? u[e] * rs : fmaf(u[e], rs, k1));
+          if constexpr (EXTRA) o[j] += add[j];
         }
         store_row_floats<T, VEC, TAIL>(dxr, column(i), cols, o);
-        if constexpr (EXTRA) {
-          if (a.dres) store_row_floats<RT, VEC, TAIL>(static_cast<RT*>(a.dres) + row * a.dres_pitch, column(i), cols, o);
-        }
+        if (a.dres) store_row_floats<RT, VEC, TAIL>(static_cast<RT*>(a.dres) + row * a.dres_pitch, column(i), cols, o);   // uniform
       }
     }
-  }
+  };
+  // (the loops' bounds are the same for the whole workgroup, so every thread reaches the reductions' barriers)
+#pragma nounroll
+  for (; base + (PF - 1) * stride + Group::kRows <= a.rows; base += PF * stride)
+    static_for<PF>([&](auto slot) { step(slot, std::false_type{}); });
+#pragma nounroll
+  for (; base < a.rows; base += PF * stride)
+    static_for<PF>([&](auto slot) { step(slot, std::true_type{}); });
   auto put = [&](float* dst, const float* acc) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (column(i) < pitch) {
+      if (!TAIL || column(i) < pitch) {
 #pragma unroll
         for (int j = 0; j < VEC; j += 4)
           st16(dst + column(i) + j, u32x4{f2u(acc[i * VEC + j]), f2u(acc[i * VEC + j + 1]), f2u(acc[i * VEC + j + 2]),
@@ -292,6 +319,151 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   if constexpr (!IS_RMS) leave(a.part_dbeta, db);
 }
 
+// The whole backward of few rows in one launch: the first `sums` workgroups form the column sums of 8 vectors of columns each,
+// from all rows, the others dx, rows side by side in a workgroup.  The partial rows that the kernel above would leave are as
+// many bytes as the rows themselves by then (512 x 5120 bf16: 13.6 us and 5.6 more for the fold; so 7).  Only where nothing
+// that is written lies over what is read.
+template <typename T, typename RT, int NV, bool EXTRA, bool IS_RMS, bool TAIL>
+__global__ __launch_bounds__(kSmallThreads)
+void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
+  constexpr int VEC = q8_vec<T, RT>(), KS = IS_RMS ? 1 : 2, LANES = 8;
+  using Words = Q8Words<VEC>;
+  __shared__ __align__(16) float red[kMaxWaves * KS];
+  const int cols = a.cols, pitch = a.blocks * kQ8Block, rows = a.rows;
+  const T* const dz = static_cast<const T*>(a.dz);
+  if (int(blockIdx.x) < sums) {
+    struct Fetched {
+      RowVec<T, VEC, true> dz;   // (the last workgroup's columns may lie past the row's end)
+      typename Words::type q;
+      uint8_t e;
+      float mu, rs;
+    };
+    const int first = int(blockIdx.x) * LANES * VEC, col = first + (int(threadIdx.x) & (LANES - 1)) * VEC;
+    const uint32_t c = uint32_t(min(col, pitch - VEC));
+    column_sums_of_few_rows<KS, VEC, LANES>(
+        rows,
+        [&](int64_t r) {
+          Fetched f;
+          f.dz.template load<true>(dz + r * a.dz_pitch, col, cols);
+          f.q = *reinterpret_cast<const typename Words::type*>(a.q + r * pitch + c);
+          f.e = a.scale[r * a.blocks + c / kQ8Block];
+          f.mu = IS_RMS ? 0.f : a.mu[r];
+          f.rs = a.rs[r];
+          return f;
+        },
+        [&](const Fetched& f, bool in, float (&acc)[KS][VEC]) {
+          float x[VEC], d[VEC];
+          f.dz.floats(d, col, cols);
+          Words::numbers(f.q, x);
+          const float step = f.rs * q8_step(f.e), shift = IS_RMS ? 0.f : -f.rs * f.mu;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float xh = IS_RMS ? x[j] * step : fmaf(x[j], step, shift);
+            const float more = fmaf(d[j], xh, acc[0][j]);
+            acc[0][j] = in ? more : acc[0][j];
+            if constexpr (KS == 2) acc[1][j] += in ? d[j] : 0.f;
+          }
+        },
+        [&](int k, int j, float sum) {
+          T* out = reinterpret_cast<T*>(k == 0 ? a.part_dgamma : a.part_dbeta);
+          if (out != nullptr && first + j < cols) Cvt<T>::store(out + first + j, sum);
+        });
+    return;
+  }
+  const int tpr = a.threads, rpb = kSmallThreads / tpr;
+  const int group = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / tpr), t = int(threadIdx.x) - group * tpr;
+  // (wavefronts that no row is left for work on the last one too and store nothing)
+  const bool idle = group >= rpb;
+  const int64_t wanted = idle ? rows : int64_t(int(blockIdx.x) - sums) * rpb + group, row = wanted < rows ? wanted : rows - 1;
+  auto column = [&](int i) { return (i * tpr + t) * VEC; };
+  const T* gp = static_cast<const T*>(a.gamma);
+  RowVec<T, VEC, TAIL> rd[NV], rg[NV];
+  [[maybe_unused]] RowVec<RT, VEC, TAIL> up[EXTRA ? NV : 1];
+  typename Words::type q[NV];
+  uint8_t e[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = uint32_t(TAIL ? min(column(i), pitch - VEC) : column(i));
+    rd[i].template load<true>(dz + row * a.dz_pitch, column(i), cols);
+    q[i] = *reinterpret_cast<const typename Words::type*>(a.q + row * pitch + c);
+    e[i] = a.scale[row * a.blocks + c / kQ8Block];
+    if (gp) rg[i].template load<true>(gp, column(i), cols);   // uniform
+    if constexpr (EXTRA) up[i].load(static_cast<const RT*>(a.dx_in) + row * a.dxin_pitch, column(i), cols);
+  }
+  const float rs = a.rs[row];
+  [[maybe_unused]] const float shift = IS_RMS ? 0.f : -rs * a.mu[row];
+  float x[NV][VEC], u[NV][VEC];
+  SumTuple<KS> s = SumTuple<KS>::identity();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float g[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g[j] = 1.f;
+    if (gp) rg[i].floats(g, column(i), cols);
+    rd[i].floats(u[i], column(i), cols);
+    Words::numbers(q[i], x[i]);
+    const float step = rs * q8_step(e[i]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {   // as in the kernel above, to the same bits
+      x[i][j] = IS_RMS ? x[i][j] * step : fmaf(x[i][j], step, shift);
+      if constexpr (TAIL) x[i][j] = column(i) + j < cols ? x[i][j] : 0.f;
+      u[i][j] *= g[j];
+      s.v[KS - 1] = fmaf(u[i][j], x[i][j], s.v[KS - 1]);
+      if constexpr (!IS_RMS) s.v[0] += u[i][j];
+    }
+  }
+  s = group_allreduce_tuple(s, red, idle ? 0 : group * (tpr >> 6), tpr >> 6);
+  if (wanted >= rows) return;
+  const float k1 = IS_RMS ? 0.f : -rs * (s.v[0] * a.inv_cols), k2 = -rs * (s.v[KS - 1] * a.inv_cols);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float o[VEC];
+    [[maybe_unused]] float add[VEC];
+    if constexpr (EXTRA) up[i].floats(add, column(i), cols);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      o[j] = fmaf(x[i][j], k2, IS_RMS ? u[i][j] * rs : fmaf(u[i][j], rs, k1));
+      if constexpr (EXTRA) o[j] += add[j];
+    }
+    store_row_floats<T, VEC, TAIL>(static_cast<T*>(a.dx0) + row * a.dx_pitch, column(i), cols, o);
+    if (a.dres) store_row_floats<RT, VEC, TAIL>(static_cast<RT*>(a.dres) + row * a.dres_pitch, column(i), cols, o);
+  }
+}
+
+template <typename T, typename RT, int NV, bool EXTRA, bool TAIL>
+static void launch_q8_norm_few(const Q8BwdArgs& a, bool is_rms, dim3 grid, int sums, hipStream_t s) {
+  profile_before(s);
+  if (is_rms) HK_LAUNCH((q8_norm_bwd_few_kernel<T, RT, NV, EXTRA, true, TAIL>), grid, dim3(kSmallThreads), 0, s, a, sums);
+  else HK_LAUNCH((q8_norm_bwd_few_kernel<T, RT, NV, EXTRA, false, TAIL>), grid, dim3(kSmallThreads), 0, s, a, sums);
+  profile_after(s);
+}
+template <typename T, typename RT>
+static int q8_norm_few(Q8BwdArgs a, bool is_rms, const Q8Shape& shape, void* dgamma, void* dbeta, hipStream_t s) {
+  constexpr int VEC = q8_vec<T, RT>();
+  a.part_dgamma = static_cast<float*>(dgamma);
+  a.part_dbeta = static_cast<float*>(dbeta);
+  const bool tail = a.cols != shape.nv * shape.lanes * VEC;
+  const int sums = (a.blocks * kQ8Block + 8 * VEC - 1) / (8 * VEC), rpb = kSmallThreads / shape.lanes;
+  const dim3 grid{unsigned(sums + (a.rows + rpb - 1) / rpb)};
+#define HK_Q8_FEW(NV)                                                                                                \
+  do {                                                                                                               \
+    if (a.dx_in) {                                                                                                   \
+      if (tail) launch_q8_norm_few<T, RT, NV, true, true>(a, is_rms, grid, sums, s);                                 \
+      else launch_q8_norm_few<T, RT, NV, true, false>(a, is_rms, grid, sums, s);                                     \
+    } else {                                                                                                         \
+      if (tail) launch_q8_norm_few<T, RT, NV, false, true>(a, is_rms, grid, sums, s);                                \
+      else launch_q8_norm_few<T, RT, NV, false, false>(a, is_rms, grid, sums, s);                                    \
+    }                                                                                                                \
+  } while (0)
+  switch (shape.nv) {
+    case 1: HK_Q8_FEW(1); break;
+    case 2: HK_Q8_FEW(2); break;
+    default: HK_Q8_FEW(4); break;
+  }
+#undef HK_Q8_FEW
+  return launch_check("q8_norm_bwd_few_kernel");
+}
+
 // the partial rows folded into dgamma / dbeta (blockIdx.y picks which)
 template <typename T, int LANES>
 __global__ __launch_bounds__(fold_threads(LANES))
@@ -304,13 +476,16 @@ void q8_norm_fold_kernel(const float* part0, const float* part1, T* out0, T* out
 template <typename T, typename RT, int NV, int LPR, bool TAIL>
 static void launch_q8_norm_fwd(const Q8FwdArgs& a, bool is_rms, hipStream_t s) {
   const dim3 grid{unsigned((a.rows + Q8Group<LPR>::kRows - 1) / Q8Group<LPR>::kRows)}, block{LPR ? 256u : unsigned(a.threads)};
+  // four workgroups of 256 threads to a compute unit where a 16-bit residual comes along: see the kernel
+  size_t lds = 0;
+  if (a.residual && LPR == 0 && a.threads == 256 && q8_vec<T, RT>() == 8) lds_bytes_for_residency(4, 256, &lds);
   profile_before(s);
   if (a.residual) {
-    if (is_rms) HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, true, true, TAIL>), grid, block, 0, s, a);
-    else HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, true, false, TAIL>), grid, block, 0, s, a);
+    if (is_rms) HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, true, true, TAIL>), grid, block, lds, s, a);
+    else HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, true, false, TAIL>), grid, block, lds, s, a);
   } else {
-    if (is_rms) HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, false, true, TAIL>), grid, block, 0, s, a);
-    else HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, false, false, TAIL>), grid, block, 0, s, a);
+    if (is_rms) HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, false, true, TAIL>), grid, block, lds, s, a);
+    else HK_LAUNCH((q8_norm_fwd_kernel<T, RT, NV, LPR, false, false, TAIL>), grid, block, lds, s, a);
   }
   profile_after(s);
 }
@@ -319,7 +494,7 @@ static void launch_q8_norm_bwd(const Q8BwdArgs& a, bool is_rms, hipStream_t s) {
   const dim3 grid{unsigned(a.grid)}, block{LPR ? 256u : unsigned(a.threads)};
   const size_t lds = LPR ? size_t(Q8Group<LPR>::kRows) * a.blocks * kQ8Block * sizeof(float) : 0;
   profile_before(s);
-  if (a.dx_in || a.dres) {
+  if (a.dx_in) {
     if (is_rms) HK_LAUNCH((q8_norm_bwd_kernel<T, RT, NV, LPR, MAXT, true, true, TAIL>), grid, block, lds, s, a);
     else HK_LAUNCH((q8_norm_bwd_kernel<T, RT, NV, LPR, MAXT, true, false, TAIL>), grid, block, lds, s, a);
   } else {
@@ -332,7 +507,7 @@ static void launch_q8_norm_bwd(const Q8BwdArgs& a, bool is_rms, hipStream_t s) {
 // WHAT: 0 forward, 1 backward
 template <typename T, typename RT, int WHAT, typename A>
 static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStream_t s) {
-  const bool tail = a.cols % VecIO<T>::N != 0;
+  const bool tail = a.cols != shape.nv * shape.lanes * q8_vec<T, RT>();   // a lane's vector may lie outside the row
 #define HK_Q8(NV, LPR)                                                                               \
   do {                                                                                               \
     if constexpr (WHAT == 0) {                                                                       \
@@ -340,9 +515,9 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
       else launch_q8_norm_fwd<T, RT, NV, LPR, false>(a, is_rms, s);                                  \
     } else {                                                                                         \
       constexpr int kMost = LPR ? 256 : 512;                                                         \
-      if (LPR == 0 && NV >= 4 && a.threads > kMost) {                                                \
-        if (tail) launch_q8_norm_bwd<T, RT, NV, LPR, LPR || NV < 4 ? kMost : 1024, true>(a, is_rms, s);  \
-        else launch_q8_norm_bwd<T, RT, NV, LPR, LPR || NV < 4 ? kMost : 1024, false>(a, is_rms, s);  \
+      if (LPR == 0 && a.threads > kMost) {                                                           \
+        if (tail) launch_q8_norm_bwd<T, RT, NV, LPR, LPR ? kMost : 1024, true>(a, is_rms, s);        \
+        else launch_q8_norm_bwd<T, RT, NV, LPR, LPR ? kMost : 1024, false>(a, is_rms, s);            \
       } else if (tail) launch_q8_norm_bwd<T, RT, NV, LPR, kMost, true>(a, is_rms, s);                \
       else launch_q8_norm_bwd<T, RT, NV, LPR, kMost, false>(a, is_rms, s);                           \
     }                                                                                                \
@@ -364,8 +539,8 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
         case 2: HK_Q8(2, 0); break;
         case 4: HK_Q8(4, 0); break;
         default:
-          HK_REQUIRE(sizeof(T) == 4 && shape.nv == 8, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
-          if constexpr (sizeof(T) == 4) HK_Q8(8, 0);
+          HK_REQUIRE((q8_vec<T, RT>() == 4) && shape.nv == 8, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
+          if constexpr (q8_vec<T, RT>() == 4) HK_Q8(8, 0);
           break;
       }
   }
@@ -384,6 +559,12 @@ template <typename T>
 int q8_norm_bwd_typed(const Q8BwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, void* dgamma, void* dbeta,
                       hipStream_t s) {
   int rc;
+  if (a.few) {
+    if constexpr (sizeof(T) == 2) {
+      if (rtype == HK_FLOAT32) return q8_norm_few<T, float>(a, is_rms, shape, dgamma, dbeta, s);
+    }
+    return q8_norm_few<T, T>(a, is_rms, shape, dgamma, dbeta, s);
+  }
   if (sizeof(T) == 2 && rtype == HK_FLOAT32) {
     if constexpr (sizeof(T) == 2) rc = launch_q8_norm<T, float, 1>(a, is_rms, shape, s);
   } else {
