@@ -48,10 +48,11 @@ struct RowVec {
       raw = u32x4{w.x, w.y, 0, 0};
     }
   }
-  __device__ __forceinline__ void floats(float* f, int c, int cols) const {
+  // full (uniform): every lane's vector lies inside the row
+  __device__ __forceinline__ void floats(float* f, int c, int cols, bool full = false) const {
     u32x4 r = raw;
     if constexpr (TAIL) {
-      if (cols >= N) {   // uniform
+      if (!full && cols >= N) {   // uniform
         const int bits = (c - min(c, cols - N)) * int(sizeof(R)) * 8;
         const uint64_t lo = uint64_t(r.y) << 32 | r.x;
         if constexpr (kWords == 2) {
@@ -103,13 +104,26 @@ __device__ __forceinline__ void store_row_floats(R* row, int c, int cols, const 
 }
 
 // The exponent field of the block that this lane's N elements belong to: the 32 / N lanes of a block are neighbours and
-// start at a multiple of their number.  Infinities and NaN have the largest field, 255.
-template <int N>
+// start at a multiple of their number.  Infinities and NaN have the largest field, 255.  ANY: a NaN may be among them (a
+// maximum of floats passes it over; integers see it, for an instruction more per element).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {   // max(|a|, |b|, c)
+  float r;
+  asm("v_max3_f32 %0, |%1|, |%2|, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int N, bool ANY = true>
 __device__ __forceinline__ uint32_t q8_exponent(const float* f) {
   static_assert(N == 4 || N == 8, "a block is 8 or 4 lanes");
   uint32_t m = 0;
+  if constexpr (ANY) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) m = max(m, f2u(f[j]) & 0x7fffffffu);
+    for (int j = 0; j < N; ++j) m = max(m, f2u(f[j]) & 0x7fffffffu);
+  } else {
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) x = max3_abs(f[j], f[j + 1], x);
+    m = f2u(x);
+  }
   m = max(m, f2u(dpp_perm<kDppXor1>(u2f(m))));
   m = max(m, f2u(dpp_perm<kDppXor2>(u2f(m))));
   if constexpr (N == 4) m = max(m, f2u(dpp_perm<kDppHalfMirror>(u2f(m))));
@@ -119,9 +133,10 @@ __device__ __forceinline__ uint32_t q8_exponent(const float* f) {
 // whole number, ties to even, whose two's complement stands in its lowest bits.
 __device__ __forceinline__ float q8_factor(uint32_t exponent) { return u2f((260u - exponent) << 23); }
 __device__ __forceinline__ uint32_t q8_encode4(const float* f, float factor) {
+  constexpr float kMagic = 12582912.f;
   uint32_t b[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = f2u(__builtin_amdgcn_fmed3f(f[j] * factor, -127.f, 127.f) + 12582912.f);
+  for (int j = 0; j < 4; ++j) b[j] = f2u(__builtin_amdgcn_fmed3f(fmaf(f[j], factor, kMagic), kMagic - 127.f, kMagic + 127.f));
   const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
   return lo | hi;
 }

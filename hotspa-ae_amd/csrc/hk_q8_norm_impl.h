@@ -42,6 +42,12 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
   const int cols = a.cols;
   auto column = [&](int i) { return (i * tpr + t) * VEC; };
 
+  // whether vector i of every lane lies inside the row (uniform; without TAIL all do)
+  auto full = [&](int i) { return !TAIL || (i + 1) * tpr * VEC <= cols; };
+
+  const T* gp = static_cast<const T*>(a.gamma);
+  const T* bp = static_cast<const T*>(a.beta);
+  RowVec<T, VEC, TAIL> g[NV], b[NV];
   float v[NV][VEC];
   {
     RowVec<T, VEC, TAIL> x[NV];
@@ -55,10 +61,10 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      x[i].floats(v[i], column(i), cols);
+      x[i].floats(v[i], column(i), cols, full(i));
       if constexpr (HAS_RES) {
         float f[VEC];
-        r[i].floats(f, column(i), cols);
+        r[i].floats(f, column(i), cols, full(i));
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] += f[j];
       }
@@ -71,6 +77,31 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
       for (int i = 0; i < NV; ++i) store_row_floats<RT, VEC, TAIL>(xo, column(i), cols, v[i]);
     }
   };
+  // the input in 8 bits, zeros behind the row's end up to the block's; before LayerNorm centres the row in place
+  auto keep = [&](float sum) {   // sum of this thread's elements: a NaN where one of them is
+    const bool nan = __builtin_expect(__builtin_amdgcn_ballot_w64(sum != sum) != 0, 0);   // uniform in a wavefront
+    int8_t* qr = a.q + row * int64_t(a.blocks) * kQ8Block;
+    uint8_t* sr = a.scale + row * int64_t(a.blocks);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t e = q8_exponent<VEC, false>(v[i]);
+      if (nan) e = q8_exponent<VEC, true>(v[i]);
+      const typename Words::type w = Words::encode(v[i], q8_factor(e));
+      const uint32_t c = uint32_t(column(i));
+      if (!TAIL || int(c) < a.blocks * kQ8Block) {
+        *reinterpret_cast<typename Words::type*>(qr + c) = w;
+        if (t % LPB == 0) sr[c / kQ8Block] = uint8_t(e);
+      }
+    }
+  };
+  auto parameters = [&] {
+    if (gp)   // uniform
+#pragma unroll
+      for (int i = 0; i < NV; ++i) g[i].template load<true>(gp, column(i), cols);
+    if (bp)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) b[i].template load<true>(bp, column(i), cols);
+  };
   float mu, rs;
   if constexpr (IS_RMS) {
     SumTuple<2> s = SumTuple<2>::identity();
@@ -78,7 +109,9 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) { s.v[0] = fmaf(v[i][j], v[i][j], s.v[0]); s.v[1] += v[i][j]; }
+    keep(s.v[0]);
     s = Group::allreduce(s, red[0], tpr);
+    parameters();
     mu = s.v[1] * a.inv_cols;
     rs = 1.0f / sqrtf(s.v[0] * a.inv_cols + a.eps);
     store_sum();
@@ -88,17 +121,28 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s.v[0] += v[i][j];
+    keep(s.v[0]);
     s = Group::allreduce(s, red[0], tpr);
+    parameters();
     mu = s.v[0] * a.inv_cols;
     store_sum();
+    // centred in place: the second sum and z take the same values
     s = SumTuple<1>::identity();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int left = cols - column(i);
+      if (full(i)) {   // uniform
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = !TAIL || j < left ? v[i][j] - mu : 0.f;
-        s.v[0] = fmaf(d, d, s.v[0]);
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] -= mu;
+          s.v[0] = fmaf(v[i][j], v[i][j], s.v[0]);
+        }
+      } else {
+        const int left = cols - column(i);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] = j < left ? v[i][j] - mu : 0.f;
+          s.v[0] = fmaf(v[i][j], v[i][j], s.v[0]);
+        }
       }
     }
     s = Group::allreduce(s, red[1], tpr);
@@ -108,37 +152,27 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     a.mu[row] = mu;
     a.rs[row] = rs;
   }
-  // the input in 8 bits; zeros behind the row's end up to the block's
-  int8_t* qr = a.q + row * int64_t(a.blocks) * kQ8Block;
-  uint8_t* sr = a.scale + row * int64_t(a.blocks);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t e = q8_exponent<VEC>(v[i]);
-    const typename Words::type w = Words::encode(v[i], q8_factor(e));
-    const int c = column(i);
-    if (!TAIL || c < a.blocks * kQ8Block) {
-      *reinterpret_cast<typename Words::type*>(qr + c) = w;
-      if (t % LPB == 0) sr[c / kQ8Block] = uint8_t(e);
-    }
-  }
   T* zr = static_cast<T*>(a.z) + row * a.z_pitch;
-  const T* gp = static_cast<const T*>(a.gamma);
-  const T* bp = static_cast<const T*>(a.beta);
-  const float shift = IS_RMS ? 0.f : mu;
+  auto finish = [&](auto has_g, auto has_b) {
+    constexpr bool HG = decltype(has_g)::value, HB = decltype(has_b)::value;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = column(i);
-    float g[VEC], b[VEC], f[VEC];
-    RowVec<T, VEC, TAIL> p;
-    if (gp) { p.template load<true>(gp, c, cols); p.floats(g, c, cols); }   // uniform
-    if (bp) { p.template load<true>(bp, c, cols); p.floats(b, c, cols); }
+    for (int i = 0; i < NV; ++i) {
+      [[maybe_unused]] float gf[VEC], bf[VEC];
+      float f[VEC];
+      if constexpr (HG) g[i].floats(gf, column(i), cols, full(i));
+      if constexpr (HB) b[i].floats(bf, column(i), cols, full(i));
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float n = rs * (v[i][j] - shift);
-      f[j] = gp ? (bp ? fmaf(g[j], n, b[j]) : g[j] * n) : (bp ? n + b[j] : n);
+      for (int j = 0; j < VEC; ++j) {
+        const float n = rs * v[i][j];
+        f[j] = HG ? (HB ? fmaf(gf[j], n, bf[j]) : gf[j] * n) : (HB ? n + bf[j] : n);
+      }
+      store_row_floats<T, VEC, TAIL>(zr, column(i), cols, f);
     }
-    store_row_floats<T, VEC, TAIL>(zr, c, cols, f);
-  }
+  };
+  if (gp && bp) finish(std::true_type{}, std::true_type{});   // uniform
+  else if (gp) finish(std::true_type{}, std::false_type{});
+  else if (bp) finish(std::false_type{}, std::true_type{});
+  else finish(std::false_type{}, std::false_type{});
 }
 
 // A persistent grid walks the rows; a thread keeps its columns' sums of dz x^ and dz, and the workgroup leaves one fp32
