@@ -82,6 +82,7 @@ NDArray wrap(const HtArray* a) {
 }
 
 Stream stream_of(const HtArray* a, int stream_index) {
+  HT_VALUE_ERROR_IF(a == nullptr) << "an array that the call cannot do without is missing";
   return Stream(device_of(a), StreamIndex(stream_index));
 }
 
@@ -517,6 +518,89 @@ int ht_vocab_parallel_cross_entropy_gradient(const HtArray* softmax, const HtArr
     hetu::impl::VocabParallelCrossEntropyGradientCuda(wrap(softmax), wrap(labels), vocab_start_index,
                                                       vocab_end_index, ignored_index, wrap(grad_loss), o,
                                                       stream_of(softmax, stream_index));
+  });
+}
+
+int ht_token_logprob(const HtArray* pred, const HtArray* token, HtArray* logprob, HtArray* entropy, HtArray* lse,
+                     HtArray* top_logprob, HtArray* top_token, int64_t ignored_index, int stream_index) {
+  return guarded([&] {
+    NDArray lp = wrap(logprob), e = wrap(entropy), l = wrap(lse), tv = wrap(top_logprob), tt = wrap(top_token);
+    hetu::impl::TokenLogProbCuda(wrap(pred), wrap(token), lp, e, l, tv, tt, ignored_index, stream_of(pred, stream_index));
+  });
+}
+
+int ht_token_logprob_gradient(const HtArray* pred, const HtArray* token, const HtArray* lse, const HtArray* entropy,
+                              const HtArray* grad_logprob, const HtArray* grad_entropy, HtArray* output,
+                              int64_t vocab_start_index, int64_t ignored_index, int stream_index) {
+  return guarded([&] {
+    NDArray o = wrap(output);
+    hetu::impl::TokenLogProbGradientCuda(wrap(pred), wrap(token), wrap(lse), wrap(entropy), wrap(grad_logprob),
+                                         wrap(grad_entropy), o, vocab_start_index, ignored_index,
+                                         stream_of(pred, stream_index));
+  });
+}
+
+int ht_vocab_parallel_logprob_stats(const HtArray* vocab_parallel_logits, const HtArray* token, HtArray* stats,
+                                    HtArray* top_value, HtArray* top_token, int64_t vocab_start_index,
+                                    int64_t ignored_index, int stream_index) {
+  return guarded([&] {
+    NDArray st = wrap(stats), tv = wrap(top_value), tt = wrap(top_token);
+    hetu::impl::VocabParallelLogProbStatsCuda(wrap(vocab_parallel_logits), wrap(token), st, tv, tt, vocab_start_index,
+                                              ignored_index, stream_of(vocab_parallel_logits, stream_index));
+  });
+}
+
+int ht_vocab_parallel_logprob_combine(const HtArray* stats, const HtArray* top_values, const HtArray* top_tokens,
+                                      const HtArray* token, int64_t ignored_index, int64_t vocab_size, HtArray* logprob,
+                                      HtArray* entropy, HtArray* lse, HtArray* top_logprob, HtArray* top_token,
+                                      int stream_index) {
+  return guarded([&] {
+    NDArray lp = wrap(logprob), e = wrap(entropy), l = wrap(lse), tv = wrap(top_logprob), tt = wrap(top_token);
+    hetu::impl::VocabParallelLogProbCombineCuda(wrap(stats), wrap(top_values), wrap(top_tokens), wrap(token), ignored_index,
+                                                vocab_size, lp, e, l, tv, tt, stream_of(stats, stream_index));
+  });
+}
+
+int ht_q8_pack(const HtArray* input, HtArray* q, HtArray* scale, int stream_index) {
+  return guarded([&] {
+    NDArray qa = wrap(q), sa = wrap(scale);
+    hetu::impl::Q8PackCuda(wrap(input), qa, sa, stream_of(input, stream_index));
+  });
+}
+
+int ht_q8_unpack(const HtArray* q, const HtArray* scale, HtArray* output, int stream_index) {
+  return guarded([&] {
+    NDArray o = wrap(output);
+    hetu::impl::Q8UnpackCuda(wrap(q), wrap(scale), o, stream_of(output, stream_index));
+  });
+}
+
+int ht_add_ln_q8_fwd(const HtArray* x0, const HtArray* residual, const HtArray* gamma, const HtArray* beta, HtArray* z,
+                     HtArray* x, HtArray* q, HtArray* scale, HtArray* mu, HtArray* rsigma, float epsilon, int is_rms_norm,
+                     int stream_index) {
+  return guarded([&] {
+    NDArray za = wrap(z), xa = wrap(x), qa = wrap(q), sa = wrap(scale), ma = wrap(mu), ra = wrap(rsigma);
+    hetu::impl::AddLnQ8FwdCuda(wrap(x0), wrap(residual), wrap(gamma), wrap(beta), za, xa, qa, sa, ma, ra, epsilon,
+                               is_rms_norm != 0, stream_of(x0, stream_index));
+  });
+}
+
+int ht_add_ln_q8_out(const HtArray* q, const HtArray* scale, const HtArray* mu, const HtArray* rsigma, const HtArray* gamma,
+                     const HtArray* beta, HtArray* z, int is_rms_norm, int stream_index) {
+  return guarded([&] {
+    NDArray za = wrap(z);
+    hetu::impl::AddLnQ8OutCuda(wrap(q), wrap(scale), wrap(mu), wrap(rsigma), wrap(gamma), wrap(beta), za, is_rms_norm != 0,
+                               stream_of(z, stream_index));
+  });
+}
+
+int ht_add_ln_q8_bwd(const HtArray* dz, const HtArray* dx, const HtArray* q, const HtArray* scale, const HtArray* mu,
+                     const HtArray* rsigma, const HtArray* gamma, HtArray* dx0, HtArray* dresidual, HtArray* dgamma,
+                     HtArray* dbeta, int is_rms_norm, int stream_index) {
+  return guarded([&] {
+    NDArray d0 = wrap(dx0), dr = wrap(dresidual), dg = wrap(dgamma), db = wrap(dbeta);
+    hetu::impl::AddLnQ8BwdCuda(wrap(dz), wrap(dx), wrap(q), wrap(scale), wrap(mu), wrap(rsigma), wrap(gamma), d0, dr, dg, db,
+                               is_rms_norm != 0, stream_of(dz, stream_index));
   });
 }
 

@@ -152,6 +152,33 @@ DECLARE_KERNEL_CUDA(SoftmaxCrossEntropySparseGradientReduced, const NDArray&, co
                     NDArray&, const int64_t, const Stream&);
 DECLARE_KERNEL_CUDA(SoftmaxCrossEntropyGradientReduced, const NDArray&, const NDArray&, const NDArray&, double,
                     NDArray&, const Stream&);
+// Log probabilities of given tokens, entropy, alternatives, their gradient and vocabulary-parallel form; activations kept in
+// 8 bits and the norm that keeps its input so (no counterparts in the reference, accelerator only).  Undefined arrays are
+// outputs left out or operands that do not exist.
+// pred, token, logprob, entropy, lse, top_logprob, top_token, ignored_index
+DECLARE_KERNEL_CUDA(TokenLogProb, const NDArray&, const NDArray&, NDArray&, NDArray&, NDArray&, NDArray&, NDArray&,
+                    const int64_t, const Stream&);
+// pred, token, lse, entropy, grad_logprob, grad_entropy, output, vocab_start_index, ignored_index
+DECLARE_KERNEL_CUDA(TokenLogProbGradient, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const NDArray&,
+                    const NDArray&, NDArray&, const int64_t, const int64_t, const Stream&);
+// vocab_parallel_logits, token, stats, top_value, top_token, vocab_start_index, ignored_index
+DECLARE_KERNEL_CUDA(VocabParallelLogProbStats, const NDArray&, const NDArray&, NDArray&, NDArray&, NDArray&, const int64_t,
+                    const int64_t, const Stream&);
+// stats, top_values, top_tokens, token, ignored_index, vocab_size, logprob, entropy, lse, top_logprob, top_token
+DECLARE_KERNEL_CUDA(VocabParallelLogProbCombine, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const int64_t,
+                    const int64_t, NDArray&, NDArray&, NDArray&, NDArray&, NDArray&, const Stream&);
+// input, q, scale  /  q, scale, output
+DECLARE_KERNEL_CUDA(Q8Pack, const NDArray&, NDArray&, NDArray&, const Stream&);
+DECLARE_KERNEL_CUDA(Q8Unpack, const NDArray&, const NDArray&, NDArray&, const Stream&);
+// x0, residual, gamma, beta, z, x, q, scale, mu, rsigma, epsilon, is_rms_norm
+DECLARE_KERNEL_CUDA(AddLnQ8Fwd, const NDArray&, const NDArray&, const NDArray&, const NDArray&, NDArray&, NDArray&, NDArray&,
+                    NDArray&, NDArray&, NDArray&, const float, bool, const Stream&);
+// q, scale, mu, rsigma, gamma, beta, z, is_rms_norm
+DECLARE_KERNEL_CUDA(AddLnQ8Out, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const NDArray&,
+                    NDArray&, bool, const Stream&);
+// dz, dx, q, scale, mu, rsigma, gamma, dx0, dresidual, dgamma, dbeta, is_rms_norm
+DECLARE_KERNEL_CUDA(AddLnQ8Bwd, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const NDArray&, const NDArray&,
+                    const NDArray&, NDArray&, NDArray&, NDArray&, NDArray&, bool, const Stream&);
 
 } // namespace impl
 } // namespace hetu

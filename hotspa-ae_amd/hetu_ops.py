@@ -230,6 +230,51 @@ def vocab_parallel_cross_entropy_gradient(softmax, labels, vocab_start, vocab_en
           int(vocab_end), int(ignored_index), grad_loss, out, stream)
 
 
+def token_logprob(pred, token, logprob, entropy, lse, top_logprob, top_token, ignored_index, stream=DEFAULT_STREAM):
+    """TokenLogProbCuda: outputs that are not wanted may be None."""
+    _call("ht_token_logprob", pred, token, logprob, entropy, lse, top_logprob, top_token, int(ignored_index), stream)
+
+
+def token_logprob_gradient(pred, token, lse, entropy, grad_logprob, grad_entropy, output, ignored_index, vocab_start=0,
+                           stream=DEFAULT_STREAM):
+    _call("ht_token_logprob_gradient", pred, token, lse, entropy, grad_logprob, grad_entropy, output, int(vocab_start),
+          int(ignored_index), stream)
+
+
+def vocab_parallel_logprob_stats(logits, token, stats, top_value, top_token, vocab_start, ignored_index,
+                                 stream=DEFAULT_STREAM):
+    _call("ht_vocab_parallel_logprob_stats", logits, token, stats, top_value, top_token, int(vocab_start),
+          int(ignored_index), stream)
+
+
+def vocab_parallel_logprob_combine(stats, top_values, top_tokens, token, ignored_index, logprob, entropy, lse, top_logprob,
+                                   top_token, vocab_size=-1, stream=DEFAULT_STREAM):
+    _call("ht_vocab_parallel_logprob_combine", stats, top_values, top_tokens, token, int(ignored_index), int(vocab_size),
+          logprob, entropy, lse, top_logprob, top_token, stream)
+
+
+def q8_pack(x, q, scale, stream=DEFAULT_STREAM):
+    _call("ht_q8_pack", x, q, scale, stream)
+
+
+def q8_unpack(q, scale, out, stream=DEFAULT_STREAM):
+    _call("ht_q8_unpack", q, scale, out, stream)
+
+
+def add_ln_q8_fwd(x0, residual, gamma, beta, z, x, q, scale, mu, rsigma, eps, is_rms, stream=DEFAULT_STREAM):
+    """AddLnQ8FwdCuda: residual, gamma, beta and x may be None."""
+    _call("ht_add_ln_q8_fwd", x0, residual, gamma, beta, z, x, q, scale, mu, rsigma, float(eps), int(is_rms), stream)
+
+
+def add_ln_q8_out(q, scale, mu, rsigma, gamma, beta, z, is_rms, stream=DEFAULT_STREAM):
+    _call("ht_add_ln_q8_out", q, scale, mu, rsigma, gamma, beta, z, int(is_rms), stream)
+
+
+def add_ln_q8_bwd(dz, dx, q, scale, mu, rsigma, gamma, dx0, dresidual, dgamma, dbeta, is_rms, stream=DEFAULT_STREAM):
+    """AddLnQ8BwdCuda: dx, gamma, dresidual, dgamma and dbeta may be None."""
+    _call("ht_add_ln_q8_bwd", dz, dx, q, scale, mu, rsigma, gamma, dx0, dresidual, dgamma, dbeta, int(is_rms), stream)
+
+
 def norm(x, out, dim, p, stream=DEFAULT_STREAM):
     _call("ht_norm", x, out, int(dim), int(p), stream)
 

@@ -476,6 +476,9 @@ PyMethodDef methods[] = {
     ENTRY(ht_softmax_cross_entropy_gradient), ENTRY(ht_softmax_cross_entropy_sparse),
     ENTRY(ht_softmax_cross_entropy_sparse_gradient), ENTRY(ht_softmax_gradient), ENTRY(ht_unary),
     ENTRY(ht_vocab_parallel_cross_entropy), ENTRY(ht_vocab_parallel_cross_entropy_gradient),
+    ENTRY(ht_token_logprob), ENTRY(ht_token_logprob_gradient), ENTRY(ht_vocab_parallel_logprob_stats),
+    ENTRY(ht_vocab_parallel_logprob_combine), ENTRY(ht_q8_pack), ENTRY(ht_q8_unpack), ENTRY(ht_add_ln_q8_fwd),
+    ENTRY(ht_add_ln_q8_out), ENTRY(ht_add_ln_q8_bwd),
 #endif
     {nullptr, nullptr, 0, nullptr}};
 

@@ -150,6 +150,33 @@ HT_API int ht_vocab_parallel_cross_entropy_gradient(const HtArray* softmax, cons
                                                     int64_t vocab_start_index, int64_t vocab_end_index,
                                                     int64_t ignored_index, const HtArray* grad_loss,
                                                     HtArray* output, int stream_index);
+/* TokenLogProbCuda, TokenLogProbGradientCuda, VocabParallelLogProbStatsCuda, VocabParallelLogProbCombineCuda: log
+ * probabilities of given tokens with entropy and alternatives (hk_token_logprob_fwd and its neighbours in hk_rowwise.h say
+ * what is computed).  An output or gradient that is not wanted is NULL. */
+HT_API int ht_token_logprob(const HtArray* pred, const HtArray* token, HtArray* logprob, HtArray* entropy, HtArray* lse,
+                            HtArray* top_logprob, HtArray* top_token, int64_t ignored_index, int stream_index);
+HT_API int ht_token_logprob_gradient(const HtArray* pred, const HtArray* token, const HtArray* lse, const HtArray* entropy,
+                                     const HtArray* grad_logprob, const HtArray* grad_entropy, HtArray* output,
+                                     int64_t vocab_start_index, int64_t ignored_index, int stream_index);
+HT_API int ht_vocab_parallel_logprob_stats(const HtArray* vocab_parallel_logits, const HtArray* token, HtArray* stats,
+                                           HtArray* top_value, HtArray* top_token, int64_t vocab_start_index,
+                                           int64_t ignored_index, int stream_index);
+HT_API int ht_vocab_parallel_logprob_combine(const HtArray* stats, const HtArray* top_values, const HtArray* top_tokens,
+                                             const HtArray* token, int64_t ignored_index, int64_t vocab_size,
+                                             HtArray* logprob, HtArray* entropy, HtArray* lse, HtArray* top_logprob,
+                                             HtArray* top_token, int stream_index);
+/* Q8PackCuda, Q8UnpackCuda, AddLnQ8FwdCuda, AddLnQ8OutCuda, AddLnQ8BwdCuda: activations kept in 8 bits and the norm that
+ * keeps its input so (hk_q8_pack, hk_add_ln_q8_fwd and their neighbours in hk_rowwise.h).  Optional arrays may be NULL. */
+HT_API int ht_q8_pack(const HtArray* input, HtArray* q, HtArray* scale, int stream_index);
+HT_API int ht_q8_unpack(const HtArray* q, const HtArray* scale, HtArray* output, int stream_index);
+HT_API int ht_add_ln_q8_fwd(const HtArray* x0, const HtArray* residual, const HtArray* gamma, const HtArray* beta, HtArray* z,
+                            HtArray* x, HtArray* q, HtArray* scale, HtArray* mu, HtArray* rsigma, float epsilon,
+                            int is_rms_norm, int stream_index);
+HT_API int ht_add_ln_q8_out(const HtArray* q, const HtArray* scale, const HtArray* mu, const HtArray* rsigma,
+                            const HtArray* gamma, const HtArray* beta, HtArray* z, int is_rms_norm, int stream_index);
+HT_API int ht_add_ln_q8_bwd(const HtArray* dz, const HtArray* dx, const HtArray* q, const HtArray* scale, const HtArray* mu,
+                            const HtArray* rsigma, const HtArray* gamma, HtArray* dx0, HtArray* dresidual, HtArray* dgamma,
+                            HtArray* dbeta, int is_rms_norm, int stream_index);
 HT_API int ht_ndarray_reduce(const HtArray* in, int red_type, const int64_t* axes, int naxes, int keepdims,
                              HtArray* out, int stream_index);
 HT_API int ht_ndarray_softmax(const HtArray* in, int64_t dim, HtArray* out, int stream_index);
