@@ -653,9 +653,21 @@ static size_t logprob_workspace(const LogprobPlan& p, int64_t rows, int top) {
   return p.splits == 1 ? 0 : size_t(p.splits) * size_t(rows) * (size_t(top) * 12 + 16);
 }
 
+// (a wavefront per row of few: it reads the parts side by side; 64 rows of 8 parts without alternatives 5.6 us instead of 12.7)
 static int launch_combine(const LogprobCombineArgs& a, hipStream_t s) {
   if (a.top || a.rows <= 1024) {
-    HK_LAUNCH((token_logprob_combine_kernel<true>), dim3(unsigned(a.rows)), dim3(64), size_t(a.n) * a.top * 12, s, a);
+    const int64_t at_once = int64_t(1) << 25;   // a launch's threads fit 32 bits
+    for (int64_t r = 0; r < a.rows; r += at_once) {
+      LogprobCombineArgs b = a;   // rows stays: it is the step between the parts
+      b.stats += r; b.tokens += r;
+      if (b.logprob) b.logprob += r;
+      if (b.entropy) b.entropy += r;
+      if (b.lse) b.lse += r;
+      if (b.out_stats) b.out_stats += r;
+      if (b.top) { b.in_value += r * b.top; b.in_token += r * b.top; b.top_value += r * b.top; b.top_token += r * b.top; }
+      HK_LAUNCH((token_logprob_combine_kernel<true>), dim3(unsigned(std::min(at_once, a.rows - r))), dim3(64),
+                size_t(a.n) * a.top * 12, s, b);
+    }
   } else {
     HK_LAUNCH((token_logprob_combine_kernel<false>), dim3(unsigned((a.rows + 255) / 256)), dim3(256), 0, s, a);
   }
@@ -703,8 +715,8 @@ static int logprob_forward(const char* name, int dtype, const void* logits, int6
   }
   const bool ragged = cols % vec != 0 || !aligned16(logits) || pitch % vec != 0;
   const bool mode1 = parts || stats;
-  // (a part per row and grid line: 65535 rows at a time)
-  const int64_t at_once = mode1 ? 65535 : rows;
+  // (a part per row and grid line: 65535 rows at a time; a launch's threads fit 32 bits)
+  const int64_t at_once = mode1 ? 65535 : (int64_t(1) << 31) / p.threads;
   HK_REQUIRE(!parts || rows <= at_once, HK_ERR_INVALID, "%s: too many rows in parts", name);
   for (int64_t r = 0; r < rows; r += at_once) {
     LogprobArgs b = a;
@@ -712,7 +724,9 @@ static int logprob_forward(const char* name, int dtype, const void* logits, int6
     const int64_t n = std::min(at_once, rows - r);
     b.logits = static_cast<const char*>(logits) + r * pitch * int64_t(dtype_size(dtype));
     b.tokens = tokens + r;
-    if (mode1) b.logprob = a.logprob + r;
+    if (a.logprob) b.logprob = a.logprob + r;
+    if (a.entropy) b.entropy = a.entropy + r;
+    if (a.lse) b.lse = a.lse + r;
     if (top && r) { b.top_value = a.top_value + r * top; b.top_token = a.top_token + r * top; }
     const dim3 grid = mode1 ? dim3(unsigned(p.splits), unsigned(n)) : dim3(unsigned(n));
     const dim3 block{unsigned(p.threads)};
@@ -821,7 +835,7 @@ int hk_token_logprob_bwd(int dtype, const void* logits, int64_t logits_pitch, co
   a.seg = (ragged ? 2 : 1) * threads * vec;
   a.segs = int((cols + a.seg - 1) / a.seg);
   hipStream_t s = as_hip(stream);
-  const int64_t at_once = std::max<int64_t>(1, 0x7fffffffLL / a.segs);   // workgroups of a launch fit 31 bits
+  const int64_t at_once = std::max<int64_t>(1, (int64_t(1) << 31) / (int64_t(a.segs) * threads));   // a launch's threads fit 32 bits
   for (int64_t r = 0; r < rows; r += at_once) {
     const int64_t n = std::min(at_once, rows - r);
     LogprobBwdArgs b = a;

@@ -35,6 +35,9 @@ __device__ __forceinline__ Q8Place q8_place(const Q8FlatArgs& a, uint32_t v, int
   return {row, int(v - row * a.row_vecs) * vec};
 }
 
+// Packing and unpacking, two vectors a thread in workgroups of 256; bound by memory.  One vector and 64 threads / so, us, of what
+// the bytes take: packing 32768 x 4096 bf16 67 / 58.6 of 59.8, 14549 x 3579 fp32 45 / 38 of 38.5; unpacking the same 62.5 / 64
+// and 52 / 44.
 template <typename T, bool TAIL, int U>
 __global__ __launch_bounds__(256)
 void q8_pack_kernel(Q8FlatArgs a) {
@@ -91,7 +94,9 @@ void q8_unpack_kernel(Q8FlatArgs a) {
   }
 }
 
-// A norm's output from its kept input, gamma rs (x8 - [mu]) + beta: a thread takes the same columns of U rows.
+// A norm's output from its kept input, gamma rs (x8 - [mu]) + beta: a thread takes the same columns of U rows, for which it
+// reads gamma and beta once (LayerNorm of 32768 x 4096 bf16, of 59.8 us that the bytes take: one row a thread 93, four
+// neighbouring vectors of a row 82, four rows 69).
 template <typename T, bool TAIL, int U>
 __global__ __launch_bounds__(256)
 void q8_norm_out_kernel(Q8FlatArgs a) {
@@ -161,6 +166,25 @@ static int each_q8_run(Q8FlatArgs a, int64_t rows, int64_t cols, size_t es, int 
     const int64_t per = (down ? 1 : per_thread) * int64_t(a.threads);
     const int rc = f(b, dim3(unsigned((vecs + per - 1) / per)));
     if (rc != HK_OK) return rc;
+  }
+  return HK_OK;
+}
+
+// f(args, rows, cols) for all rows at once, or for runs of whole blocks of each row where the offsets inside one pass 32 bits
+template <typename F>
+static int each_q8_piece(const Q8FlatArgs& a, int64_t rows, int64_t cols, size_t es, F&& f) {
+  constexpr int64_t kRun = int64_t(1) << 28;
+  if (cols <= kRun) return f(a, rows, cols);
+  for (int64_t r = 0; r < rows; ++r) {
+    for (int64_t c = 0; c < cols; c += kRun) {
+      Q8FlatArgs b = a;
+      if (b.x) b.x = static_cast<const char*>(a.x) + (r * a.pitch + c) * int64_t(es);
+      if (b.out) b.out = static_cast<char*>(a.out) + (r * a.pitch + c) * int64_t(es);
+      b.q = a.q + r * q8_blocks(cols) * kQ8Block + c;
+      b.scale = a.scale + r * q8_blocks(cols) + c / kQ8Block;
+      const int rc = f(b, 1, std::min(kRun, cols - c));
+      if (rc != HK_OK) return rc;
+    }
   }
   return HK_OK;
 }
@@ -257,6 +281,7 @@ static bool q8_apart(const Q8BwdArgs& a, const void* dgamma, const void* dbeta, 
                 Span{a.q, rows * a.blocks * kQ8Block}, Span{a.scale, rows * a.blocks}, Span{a.mu, rows * 4}, Span{a.rs, rows * 4}});
 }
 
+constexpr int64_t kQ8MaxRow = int64_t(1) << 40;   // columns of a row to pack
 static bool q8_dtype(int dtype) { return dtype == HK_FLOAT32 || dtype == HK_BFLOAT16 || dtype == HK_FLOAT16; }
 
 #define HK_Q8_TYPED(dtype, call)                      \
@@ -271,30 +296,34 @@ extern "C" {
 int hk_q8_pack(int dtype, const void* x, int64_t x_pitch, int8_t* q, uint8_t* scale, int64_t rows, int64_t cols,
                hkStream_t stream) {
   HK_REQUIRE(q8_dtype(dtype), HK_ERR_UNSUPPORTED, "hk_q8_pack: not implemented for dtype %d", dtype);
-  HK_REQUIRE(rows >= 0 && cols >= 0 && cols <= 0x7fffff00LL, HK_ERR_INVALID, "hk_q8_pack: bad shape");
+  HK_REQUIRE(rows >= 0 && cols >= 0 && cols <= kQ8MaxRow, HK_ERR_INVALID, "hk_q8_pack: bad shape");
   if (rows == 0 || cols == 0) return HK_OK;
   HK_REQUIRE(x && q && scale, HK_ERR_INVALID, "hk_q8_pack: null input/output");
   HK_REQUIRE(x_pitch >= cols, HK_ERR_INVALID, "hk_q8_pack: row pitch below the columns");
   HK_REQUIRE((reinterpret_cast<uintptr_t>(q) & 7u) == 0, HK_ERR_INVALID, "hk_q8_pack: q must lie on an 8-byte boundary");
   Q8FlatArgs a{};
   a.x = x; a.pitch = x_pitch; a.q = q; a.scale = scale;
-#define HK_CALL_PACK(T) q8_pack_typed<T>(a, rows, cols, as_hip(stream))
-  return HK_Q8_TYPED(dtype, HK_CALL_PACK);
+#define HK_CALL_PACK(T) q8_pack_typed<T>(b, n, m, as_hip(stream))
+  return each_q8_piece(a, rows, cols, dtype_size(dtype), [&](const Q8FlatArgs& b, int64_t n, int64_t m) {
+    return HK_Q8_TYPED(dtype, HK_CALL_PACK);
+  });
 #undef HK_CALL_PACK
 }
 
 int hk_q8_unpack(int dtype, const int8_t* q, const uint8_t* scale, void* out, int64_t out_pitch, int64_t rows, int64_t cols,
                  hkStream_t stream) {
   HK_REQUIRE(q8_dtype(dtype), HK_ERR_UNSUPPORTED, "hk_q8_unpack: not implemented for dtype %d", dtype);
-  HK_REQUIRE(rows >= 0 && cols >= 0 && cols <= 0x7fffff00LL, HK_ERR_INVALID, "hk_q8_unpack: bad shape");
+  HK_REQUIRE(rows >= 0 && cols >= 0 && cols <= kQ8MaxRow, HK_ERR_INVALID, "hk_q8_unpack: bad shape");
   if (rows == 0 || cols == 0) return HK_OK;
   HK_REQUIRE(out && q && scale, HK_ERR_INVALID, "hk_q8_unpack: null input/output");
   HK_REQUIRE(out_pitch >= cols, HK_ERR_INVALID, "hk_q8_unpack: row pitch below the columns");
   HK_REQUIRE((reinterpret_cast<uintptr_t>(q) & 7u) == 0, HK_ERR_INVALID, "hk_q8_unpack: q must lie on an 8-byte boundary");
   Q8FlatArgs a{};
   a.out = out; a.pitch = out_pitch; a.q = const_cast<int8_t*>(q); a.scale = const_cast<uint8_t*>(scale);
-#define HK_CALL_UNPACK(T) q8_unpack_typed<T>(a, rows, cols, as_hip(stream))
-  return HK_Q8_TYPED(dtype, HK_CALL_UNPACK);
+#define HK_CALL_UNPACK(T) q8_unpack_typed<T>(b, n, m, as_hip(stream))
+  return each_q8_piece(a, rows, cols, dtype_size(dtype), [&](const Q8FlatArgs& b, int64_t n, int64_t m) {
+    return HK_Q8_TYPED(dtype, HK_CALL_UNPACK);
+  });
 #undef HK_CALL_UNPACK
 }
 

@@ -9,6 +9,8 @@
 
 #include "hk_q8.h"
 
+#include <algorithm>
+
 namespace hk {
 
 // how a thread group holds a row: LPR lanes of a wavefront, or a workgroup (LPR == 0)
@@ -28,7 +30,10 @@ struct Q8Group {
 };
 
 // One pass: the row stays in registers, two reductions (one for RMSNorm), then z.  The sum goes out after the first
-// reduction: it may lie over the residual, and every lane has read its part of the row by then.
+// reduction: it may lie over the residual, and every lane has read its part of the row by then.  The 8 bits go out before it:
+// they need no statistics, and nothing waits for them.  Bound by memory (32768 x 4096 bf16, us here / what the bytes take:
+// RMSNorm 102 / 99, with a bf16 residual 182 / 178, with one in fp32 274 / 257; LayerNorm of 16384 x 5120 68 / 62); odd widths
+// pay for loads that begin on any element and for the row's last vector (9000 x 3579 bf16: 38 / 24).
 template <typename T, typename RT, int NV, int LPR, bool HAS_RES, bool IS_RMS, bool TAIL>
 __global__ __launch_bounds__(LPR ? 256 : 1024)
 void q8_norm_fwd_kernel(Q8FwdArgs a) {
@@ -176,15 +181,11 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
 }
 
 // A persistent grid walks the rows; a thread keeps its columns' sums of dz x^ and dz, and the workgroup leaves one fp32
-// partial row of each.  PF rows' loads are under way while a row is worked on (a ring of register slots; no load sits in a
-// branch).  EXTRA: an upstream gradient comes in.
-// MAXT: the most threads of a workgroup; above 512 the register budget is half of what the widest rows would take.
-#ifndef Q8_PF
-#define Q8_PF 1
-#endif
-template <int NV, bool EXTRA, int MAXT>
-constexpr int q8_prefetch() { return MAXT > 512 ? 1 : NV <= 2 ? Q8_PF : NV == 4 ? (Q8_PF > 1 ? 2 : 1) : 1; }
-template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, bool TAIL, int PF = q8_prefetch<NV, EXTRA, MAXT>()>
+// partial row of each.  The next row's loads are under way while a row is worked on, and none sits in a branch (two and three
+// rows ahead, RMSNorm of 32768 x 4096 bf16 with an upstream gradient: 200 and 204 us instead of 196).  Bound by memory: 178 us is
+// what the bytes take.  EXTRA: an upstream gradient comes in.  MAXT: the most threads of a workgroup; above 512 the register
+// budget is half of what the widest rows would take.
+template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, bool TAIL>
 __global__ __launch_bounds__(MAXT)
 void q8_norm_bwd_kernel(Q8BwdArgs a) {
   constexpr int VEC = q8_vec<T, RT>(), NE = NV * VEC;
@@ -221,19 +222,18 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
     dg[e] = 0.f;
     if constexpr (!IS_RMS) db[e] = 0.f;
   }
-  struct Slot {
+  struct {
     RowVec<T, VEC, TAIL> dz[NV];
     RowVec<RT, VEC, TAIL> up[EXTRA ? NV : 1];
     typename Words::type q[NV];
     uint8_t e[NV];
     float mu, rs;
-  } next[PF];
+  } next;
   const int64_t last = a.rows - 1;
-  auto issue = [&](auto slot, int64_t r) {   // a row past the end reads the last one, which is then not used
-    Slot& to = next[decltype(slot)::value];
+  auto issue = [&](int64_t r) {   // a row past the end reads the last one, which is then not used
     const int64_t rc = r < last ? r : last;
-    to.rs = a.rs[rc];
-    if constexpr (!IS_RMS) to.mu = a.mu[rc];
+    next.rs = a.rs[rc];
+    if constexpr (!IS_RMS) next.mu = a.mu[rc];
     const T* dr = static_cast<const T*>(a.dz) + rc * a.dz_pitch;
     const int8_t* qr = a.q + rc * int64_t(pitch);
     const uint8_t* sr = a.scale + rc * int64_t(a.blocks);
@@ -241,35 +241,34 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = uint32_t(TAIL ? min(column(i), pitch - VEC) : column(i));
-      to.dz[i].load(dr, column(i), cols);
-      to.q[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Words::type*>(qr + c));
-      to.e[i] = sr[c / kQ8Block];
-      if constexpr (EXTRA) to.up[i].load(ur, column(i), cols);
+      next.dz[i].load(dr, column(i), cols);
+      next.q[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Words::type*>(qr + c));
+      next.e[i] = sr[c / kQ8Block];
+      if constexpr (EXTRA) next.up[i].load(ur, column(i), cols);
     }
   };
   const int64_t stride = int64_t(a.grid) * Group::kRows;
   int64_t base = int64_t(blockIdx.x) * Group::kRows;
   int parity = 0;
-  static_for<PF>([&](auto slot) { issue(slot, base + group + decltype(slot)::value * stride); });
-  // GUARDED: the slot's row may not exist (the tail)
-  auto step = [&](auto slot, auto guarded) {
+  issue(base + group);
+  // guarded: the row may not exist (the tail)
+  auto step = [&](auto guarded) {
     constexpr bool GUARD = decltype(guarded)::value;
-    Slot& in = next[decltype(slot)::value];
-    const int64_t row = base + group + decltype(slot)::value * stride;
+    const int64_t row = base + group;
     const bool valid = !GUARD || row < a.rows;
     float x[NE], u[NE];
     [[maybe_unused]] RowVec<RT, VEC, TAIL> up[EXTRA ? NV : 1];   // (packed until it is added)
-    const float rs = in.rs;
-    [[maybe_unused]] const float shift = IS_RMS ? 0.f : -rs * in.mu;
+    const float rs = next.rs;
+    [[maybe_unused]] const float shift = IS_RMS ? 0.f : -rs * next.mu;
     float step_of[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      in.dz[i].floats(&u[i * VEC], column(i), cols);
-      Words::numbers(in.q[i], &x[i * VEC]);
-      step_of[i] = rs * q8_step(in.e[i]);   // (a power of two: exact)
-      if constexpr (EXTRA) up[i] = in.up[i];
+      next.dz[i].floats(&u[i * VEC], column(i), cols);
+      Words::numbers(next.q[i], &x[i * VEC]);
+      step_of[i] = rs * q8_step(next.e[i]);   // (a power of two: exact)
+      if constexpr (EXTRA) up[i] = next.up[i];
     }
-    issue(slot, row + PF * stride);
+    issue(row + stride);
     SumTuple<KS> s = SumTuple<KS>::identity();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -314,11 +313,8 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   };
   // (the loops' bounds are the same for the whole workgroup, so every thread reaches the reductions' barriers)
 #pragma nounroll
-  for (; base + (PF - 1) * stride + Group::kRows <= a.rows; base += PF * stride)
-    static_for<PF>([&](auto slot) { step(slot, std::false_type{}); });
-#pragma nounroll
-  for (; base < a.rows; base += PF * stride)
-    static_for<PF>([&](auto slot) { step(slot, std::true_type{}); });
+  for (; base + Group::kRows <= a.rows; base += stride) step(std::false_type{});
+  if (base < a.rows) step(std::true_type{});
   auto put = [&](float* dst, const float* acc) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -355,8 +351,8 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
 
 // The whole backward of few rows in one launch: the first `sums` workgroups form the column sums of 8 vectors of columns each,
 // from all rows, the others dx, rows side by side in a workgroup.  The partial rows that the kernel above would leave are as
-// many bytes as the rows themselves by then (512 x 5120 bf16: 13.6 us and 5.6 more for the fold; so 7).  Only where nothing
-// that is written lies over what is read.
+// many bytes as the rows themselves by then (LayerNorm of 512 x 4096 bf16: 16.8 us with them and their fold, 5.2 so).  Only
+// where nothing that is written lies over what is read.
 template <typename T, typename RT, int NV, bool EXTRA, bool IS_RMS, bool TAIL>
 __global__ __launch_bounds__(kSmallThreads)
 void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
@@ -510,7 +506,8 @@ void q8_norm_fold_kernel(const float* part0, const float* part1, T* out0, T* out
 template <typename T, typename RT, int NV, int LPR, bool TAIL>
 static void launch_q8_norm_fwd(const Q8FwdArgs& a, bool is_rms, hipStream_t s) {
   const dim3 grid{unsigned((a.rows + Q8Group<LPR>::kRows - 1) / Q8Group<LPR>::kRows)}, block{LPR ? 256u : unsigned(a.threads)};
-  // four workgroups of 256 threads to a compute unit where a 16-bit residual comes along: see the kernel
+  // four workgroups of 256 threads to a compute unit where a 16-bit residual comes along: more of them read and write more rows
+  // at once than memory takes well (RMSNorm of 32768 x 4096 bf16: 202 us without the limit, 191 with it)
   size_t lds = 0;
   if (a.residual && LPR == 0 && a.threads == 256 && q8_vec<T, RT>() == 8) lds_bytes_for_residency(4, 256, &lds);
   profile_before(s);
@@ -582,12 +579,31 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
   return launch_check(WHAT == 0 ? "q8_norm_fwd_kernel" : "q8_norm_bwd_kernel");
 }
 
+template <typename T, typename RT>
+static int q8_norm_fwd_runs(const Q8FwdArgs& a, bool is_rms, const Q8Shape& shape, hipStream_t s) {
+  const int64_t at_once = rows_of_a_launch(shape.lanes);
+  for (int64_t r = 0; r < a.rows; r += at_once) {
+    Q8FwdArgs b = a;
+    b.rows = int(std::min<int64_t>(at_once, a.rows - r));
+    b.x0 = static_cast<const T*>(a.x0) + r * a.x0_pitch;
+    b.z = static_cast<T*>(a.z) + r * a.z_pitch;
+    if (b.residual) b.residual = static_cast<const RT*>(a.residual) + r * a.res_pitch;
+    if (b.x_out) b.x_out = static_cast<RT*>(a.x_out) + r * a.xout_pitch;
+    b.q = a.q + r * int64_t(a.blocks) * kQ8Block;
+    b.scale = a.scale + r * a.blocks;
+    b.mu = a.mu + r;
+    b.rs = a.rs + r;
+    const int rc = launch_q8_norm<T, RT, 0>(b, is_rms, shape, s);
+    if (rc != HK_OK) return rc;
+  }
+  return HK_OK;
+}
 template <typename T>
 int q8_norm_fwd_typed(const Q8FwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (rtype == HK_FLOAT32) return launch_q8_norm<T, float, 0>(a, is_rms, shape, s);
+    if (rtype == HK_FLOAT32) return q8_norm_fwd_runs<T, float>(a, is_rms, shape, s);
   }
-  return launch_q8_norm<T, T, 0>(a, is_rms, shape, s);
+  return q8_norm_fwd_runs<T, T>(a, is_rms, shape, s);
 }
 template <typename T>
 int q8_norm_bwd_typed(const Q8BwdArgs& a, int rtype, bool is_rms, const Q8Shape& shape, void* dgamma, void* dbeta,
