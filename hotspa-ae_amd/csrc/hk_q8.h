@@ -15,10 +15,13 @@ inline int64_t q8_blocks(int64_t cols) { return (cols + kQ8Block - 1) / kQ8Block
 // A row's columns [c, c + N) of R as floats, c a multiple of N; 0 past the row's end: one load of 16 bytes, or of 8 where a
 // 16-bit operand goes along with an fp32 one (neighbouring lanes then read neighbouring memory in both: a residual stream in
 // fp32 beside bf16 rows, read as two 16-byte loads 32 bytes apart: the forward norm of 32768 x 4096 in 430 us instead of
-// 284).  TAIL: the row may end before or inside a vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector
-// inside the row and none sits in a branch; without it every vector lies inside.  raw is the load, floats() what comes of it.
+// 284).  kTail: the row may end before or inside a vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector
+// inside the row and none sits in a branch; kWhole: every vector lies inside; kShort: the row may be shorter than a load, a
+// variant of its own, since the branch for it makes the compiler wait for loads that are under way.  raw is the load, floats()
+// what comes of it.
 typedef u32x2 u32x2_on2 __attribute__((aligned(2)));
-template <typename R, int N, bool TAIL>
+constexpr int kWhole = 0, kTail = 1, kShort = 2;
+template <typename R, int N, int TAIL>
 struct RowVec {
   static constexpr int kWords = N * int(sizeof(R)) / 4;
   static_assert(kWords == 4 || kWords == 2, "one load of 16 or 8 bytes");
@@ -26,7 +29,7 @@ struct RowVec {
   // row: any element boundary; one of cols elements, cols >= 1
   template <bool KEEP = false>   // KEEP: read by many workgroups
   __device__ __forceinline__ void load(const R* row, int c, int cols) {
-    if (TAIL && cols < N) {   // uniform: a row shorter than a load
+    if (TAIL == kShort && cols < N) {   // uniform
       float f[8] = {};
       if (c == 0) {
 #pragma unroll
@@ -52,7 +55,7 @@ struct RowVec {
   __device__ __forceinline__ void floats(float* f, int c, int cols, bool full = false) const {
     u32x4 r = raw;
     if constexpr (TAIL) {
-      if (!full && cols >= N) {   // uniform
+      if (!full && (TAIL != kShort || cols >= N)) {   // uniform
         const int bits = (c - min(c, cols - N)) * int(sizeof(R)) * 8;
         const uint64_t lo = uint64_t(r.y) << 32 | r.x;
         if constexpr (kWords == 2) {
@@ -78,7 +81,7 @@ struct RowVec {
 };
 
 // stores N floats as R at columns [c, c + N) of a row, those inside it
-template <typename R, int N, bool TAIL>
+template <typename R, int N, int TAIL>
 __device__ __forceinline__ void store_row_floats(R* row, int c, int cols, const float* f) {
   constexpr int kWords = N * int(sizeof(R)) / 4;
   float e[8];

@@ -38,7 +38,7 @@ __device__ __forceinline__ Q8Place q8_place(const Q8FlatArgs& a, uint32_t v, int
 // Packing and unpacking, two vectors a thread in workgroups of 256; bound by memory.  One vector and 64 threads / so, us, of what
 // the bytes take: packing 32768 x 4096 bf16 67 / 58.6 of 59.8, 14549 x 3579 fp32 45 / 38 of 38.5; unpacking the same 62.5 / 64
 // and 52 / 44.
-template <typename T, bool TAIL, int U>
+template <typename T, int TAIL, int U>
 __global__ __launch_bounds__(256)
 void q8_pack_kernel(Q8FlatArgs a) {
   constexpr int VEC = VecIO<T>::N, LPB = kQ8Block / VEC;
@@ -66,7 +66,7 @@ void q8_pack_kernel(Q8FlatArgs a) {
   }
 }
 
-template <typename T, bool TAIL, int U>
+template <typename T, int TAIL, int U>
 __global__ __launch_bounds__(256)
 void q8_unpack_kernel(Q8FlatArgs a) {
   constexpr int VEC = VecIO<T>::N, LPB = kQ8Block / VEC;
@@ -97,7 +97,7 @@ void q8_unpack_kernel(Q8FlatArgs a) {
 // A norm's output from its kept input, gamma rs (x8 - [mu]) + beta: a thread takes the same columns of U rows, for which it
 // reads gamma and beta once (LayerNorm of 32768 x 4096 bf16, of 59.8 us that the bytes take: one row a thread 93, four
 // neighbouring vectors of a row 82, four rows 69).
-template <typename T, bool TAIL, int U>
+template <typename T, int TAIL, int U>
 __global__ __launch_bounds__(256)
 void q8_norm_out_kernel(Q8FlatArgs a) {
   constexpr int VEC = VecIO<T>::N, LPB = kQ8Block / VEC;
@@ -192,8 +192,9 @@ static int each_q8_piece(const Q8FlatArgs& a, int64_t rows, int64_t cols, size_t
 #define HK_Q8_LAUNCH(KERNEL)                                                                          \
   do {                                                                                                \
     profile_before(s);                                                                                \
-    if (cols % kQ8Block) HK_LAUNCH((KERNEL<T, true, U>), grid, dim3(b.threads), 0, s, b);          \
-    else HK_LAUNCH((KERNEL<T, false, U>), grid, dim3(b.threads), 0, s, b);                            \
+    if (cols % kQ8Block == 0) HK_LAUNCH((KERNEL<T, kWhole, U>), grid, dim3(b.threads), 0, s, b);      \
+    else if (cols >= VecIO<T>::N) HK_LAUNCH((KERNEL<T, kTail, U>), grid, dim3(b.threads), 0, s, b);   \
+    else HK_LAUNCH((KERNEL<T, kShort, U>), grid, dim3(b.threads), 0, s, b);                           \
     profile_after(s);                                                                                 \
   } while (0)
 template <typename T>

@@ -22,6 +22,12 @@ struct Q8Group {
     return LPR == 0 ? 0 : LPR == kWave ? wave_index() : int(threadIdx.x) / LPR;
   }
   static constexpr int kRows = LPR ? 256 / (LPR ? LPR : 1) : 1;   // rows of a workgroup
+  // the first column behind the i-th vectors of this wavefront's lanes (uniform)
+  template <int VEC>
+  static __device__ __forceinline__ int wave_end(int i, int threads) {
+    if constexpr (LPR) return (i + 1) * LPR * VEC;
+    else return (i * threads + (wave_index() + 1) * kWave) * VEC;
+  }
   template <typename P>
   static __device__ __forceinline__ P allreduce(P p, float* red, int threads) {
     if constexpr (LPR == 0) return group_allreduce_tuple(p, red, 0, threads >> 6);
@@ -33,8 +39,9 @@ struct Q8Group {
 // reduction: it may lie over the residual, and every lane has read its part of the row by then.  The 8 bits go out before it:
 // they need no statistics, and nothing waits for them.  Bound by memory (32768 x 4096 bf16, us here / what the bytes take:
 // RMSNorm 102 / 99, with a bf16 residual 182 / 178, with one in fp32 274 / 257; LayerNorm of 16384 x 5120 68 / 62); odd widths
-// pay for loads that begin on any element and for the row's last vector (9000 x 3579 bf16: 38 / 24).
-template <typename T, typename RT, int NV, int LPR, bool HAS_RES, bool IS_RMS, bool TAIL>
+// pay for loads and stores that begin on any element (LayerNorm of 9000 rows bf16: 29.5 at 3584 columns, 34.5 at 3579; 30.0 at
+// 3579 with the rows on 16-byte boundaries).
+template <typename T, typename RT, int NV, int LPR, bool HAS_RES, bool IS_RMS, int TAIL>
 __global__ __launch_bounds__(LPR ? 256 : 1024)
 void q8_norm_fwd_kernel(Q8FwdArgs a) {
   constexpr int VEC = q8_vec<T, RT>(), LPB = kQ8Block / VEC;
@@ -47,8 +54,8 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
   const int cols = a.cols;
   auto column = [&](int i) { return (i * tpr + t) * VEC; };
 
-  // whether vector i of every lane lies inside the row (uniform; without TAIL all do)
-  auto full = [&](int i) { return !TAIL || (i + 1) * tpr * VEC <= cols; };
+  // whether vector i of the wavefront's lanes lies inside the row (without TAIL all do)
+  auto full = [&](int i) { return !TAIL || Group::template wave_end<VEC>(i, tpr) <= cols; };
 
   const T* gp = static_cast<const T*>(a.gamma);
   const T* bp = static_cast<const T*>(a.beta);
@@ -185,7 +192,7 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
 // rows ahead, RMSNorm of 32768 x 4096 bf16 with an upstream gradient: 200 and 204 us instead of 196).  Bound by memory: 178 us is
 // what the bytes take.  EXTRA: an upstream gradient comes in.  MAXT: the most threads of a workgroup; above 512 the register
 // budget is half of what the widest rows would take.
-template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, bool TAIL>
+template <typename T, typename RT, int NV, int LPR, int MAXT, bool EXTRA, bool IS_RMS, int TAIL>
 __global__ __launch_bounds__(MAXT)
 void q8_norm_bwd_kernel(Q8BwdArgs a) {
   constexpr int VEC = q8_vec<T, RT>(), NE = NV * VEC;
@@ -197,6 +204,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   const int tpr = Group::count(a.threads), t = Group::lane(), group = Group::group();
   const int cols = a.cols, pitch = a.blocks * kQ8Block;
   auto column = [&](int i) { return (i * tpr + t) * VEC; };
+  auto full = [&](int i) { return !TAIL || Group::template wave_end<VEC>(i, tpr) <= cols; };
 
   float dg[NE];
   [[maybe_unused]] float db[IS_RMS ? 1 : NE];
@@ -263,7 +271,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
     float step_of[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      next.dz[i].floats(&u[i * VEC], column(i), cols);
+      next.dz[i].floats(&u[i * VEC], column(i), cols, full(i));
       Words::numbers(next.q[i], &x[i * VEC]);
       step_of[i] = rs * q8_step(next.e[i]);   // (a power of two: exact)
       if constexpr (EXTRA) up[i] = next.up[i];
@@ -273,16 +281,20 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float g[VEC];
-      if constexpr (kPacked) gm[i].floats(g, gp ? column(i) : 0, gp ? cols : VEC);
+      if constexpr (kPacked) gm[i].floats(g, gp ? column(i) : 0, gp ? cols : VEC, full(i));
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) if constexpr (!kPacked) g[j] = gf[i * VEC + j];
+      for (int j = 0; j < VEC; ++j) {
+        if constexpr (!kPacked) g[j] = gf[i * VEC + j];
+        x[i * VEC + j] = IS_RMS ? x[i * VEC + j] * step_of[i] : fmaf(x[i * VEC + j], step_of[i], shift);
+      }
+      // (nothing past the row's end, where another column's value or a NaN block's may stand)
+      if (!full(i))   // uniform
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) x[i * VEC + j] = column(i) + j < cols ? x[i * VEC + j] : 0.f;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const int e = i * VEC + j;
         const float dz = valid ? u[e] : 0.f;           // 0 past the row's end
-        x[e] = IS_RMS ? x[e] * step_of[i] : fmaf(x[e], step_of[i], shift);
-        // (nothing past the row's end, where another column's value or a NaN block's may stand)
-        if constexpr (TAIL) x[e] = column(i) + j < cols ? x[e] : 0.f;
         dg[e] = fmaf(dz, x[e], dg[e]);
         if constexpr (!IS_RMS) db[e] += dz;
         u[e] = dz * g[j];
@@ -299,7 +311,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
       for (int i = 0; i < NV; ++i) {
         float o[VEC];
         [[maybe_unused]] float add[VEC];
-        if constexpr (EXTRA) up[i].floats(add, column(i), cols);
+        if constexpr (EXTRA) up[i].floats(add, column(i), cols, full(i));
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int e = i * VEC + j;
@@ -353,7 +365,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
 // from all rows, the others dx, rows side by side in a workgroup.  The partial rows that the kernel above would leave are as
 // many bytes as the rows themselves by then (LayerNorm of 512 x 4096 bf16: 16.8 us with them and their fold, 5.2 so).  Only
 // where nothing that is written lies over what is read.
-template <typename T, typename RT, int NV, bool EXTRA, bool IS_RMS, bool TAIL>
+template <typename T, typename RT, int NV, bool EXTRA, bool IS_RMS, int TAIL>
 __global__ __launch_bounds__(kSmallThreads)
 void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
   constexpr int VEC = q8_vec<T, RT>(), KS = IS_RMS ? 1 : 2, LANES = 8;
@@ -363,7 +375,7 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
   const T* const dz = static_cast<const T*>(a.dz);
   if (int(blockIdx.x) < sums) {
     struct Fetched {
-      RowVec<T, VEC, true> dz;   // (the last workgroup's columns may lie past the row's end)
+      RowVec<T, VEC, kTail> dz;   // (the last workgroup's columns may lie past the row's end)
       typename Words::type q;
       uint8_t e;
       float mu, rs;
@@ -406,6 +418,7 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
   const bool idle = group >= rpb;
   const int64_t wanted = idle ? rows : int64_t(int(blockIdx.x) - sums) * rpb + group, row = wanted < rows ? wanted : rows - 1;
   auto column = [&](int i) { return (i * tpr + t) * VEC; };
+  auto full = [&](int i) { return !TAIL || (i * tpr + (__builtin_amdgcn_readfirstlane(t) | 63) + 1) * VEC <= cols; };   // as above
   const T* gp = static_cast<const T*>(a.gamma);
   RowVec<T, VEC, TAIL> rd[NV], rg[NV];
   [[maybe_unused]] RowVec<RT, VEC, TAIL> up[EXTRA ? NV : 1];
@@ -429,14 +442,14 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
     float g[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) g[j] = 1.f;
-    if (gp) rg[i].floats(g, column(i), cols);
-    rd[i].floats(u[i], column(i), cols);
+    if (gp) rg[i].floats(g, column(i), cols, full(i));
+    rd[i].floats(u[i], column(i), cols, full(i));
     Words::numbers(q[i], x[i]);
     const float step = rs * q8_step(e[i]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {   // as in the kernel above, to the same bits
       x[i][j] = IS_RMS ? x[i][j] * step : fmaf(x[i][j], step, shift);
-      if constexpr (TAIL) x[i][j] = column(i) + j < cols ? x[i][j] : 0.f;
+      if (TAIL && !full(i)) x[i][j] = column(i) + j < cols ? x[i][j] : 0.f;
       u[i][j] *= g[j];
       s.v[KS - 1] = fmaf(u[i][j], x[i][j], s.v[KS - 1]);
       if constexpr (!IS_RMS) s.v[0] += u[i][j];
@@ -449,7 +462,7 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
   for (int i = 0; i < NV; ++i) {
     float o[VEC];
     [[maybe_unused]] float add[VEC];
-    if constexpr (EXTRA) up[i].floats(add, column(i), cols);
+    if constexpr (EXTRA) up[i].floats(add, column(i), cols, full(i));
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       o[j] = fmaf(x[i][j], k2, IS_RMS ? u[i][j] * rs : fmaf(u[i][j], rs, k1));
@@ -460,7 +473,7 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
   }
 }
 
-template <typename T, typename RT, int NV, bool EXTRA, bool TAIL>
+template <typename T, typename RT, int NV, bool EXTRA, int TAIL>
 static void launch_q8_norm_few(const Q8BwdArgs& a, bool is_rms, dim3 grid, int sums, hipStream_t s) {
   profile_before(s);
   if (is_rms) HK_LAUNCH((q8_norm_bwd_few_kernel<T, RT, NV, EXTRA, true, TAIL>), grid, dim3(kSmallThreads), 0, s, a, sums);
@@ -478,11 +491,11 @@ static int q8_norm_few(Q8BwdArgs a, bool is_rms, const Q8Shape& shape, void* dga
 #define HK_Q8_FEW(NV)                                                                                                \
   do {                                                                                                               \
     if (a.dx_in) {                                                                                                   \
-      if (tail) launch_q8_norm_few<T, RT, NV, true, true>(a, is_rms, grid, sums, s);                                 \
-      else launch_q8_norm_few<T, RT, NV, true, false>(a, is_rms, grid, sums, s);                                     \
+      if (tail) launch_q8_norm_few<T, RT, NV, true, kTail>(a, is_rms, grid, sums, s);                                \
+      else launch_q8_norm_few<T, RT, NV, true, kWhole>(a, is_rms, grid, sums, s);                                    \
     } else {                                                                                                         \
-      if (tail) launch_q8_norm_few<T, RT, NV, false, true>(a, is_rms, grid, sums, s);                                \
-      else launch_q8_norm_few<T, RT, NV, false, false>(a, is_rms, grid, sums, s);                                    \
+      if (tail) launch_q8_norm_few<T, RT, NV, false, kTail>(a, is_rms, grid, sums, s);                               \
+      else launch_q8_norm_few<T, RT, NV, false, kWhole>(a, is_rms, grid, sums, s);                                   \
     }                                                                                                                \
   } while (0)
   switch (shape.nv) {
@@ -503,7 +516,7 @@ void q8_norm_fold_kernel(const float* part0, const float* part1, T* out0, T* out
   if (int(threadIdx.x) < 4 * LANES && c < cols) Cvt<T>::store((blockIdx.y == 0 ? out0 : out1) + c, s);
 }
 
-template <typename T, typename RT, int NV, int LPR, bool TAIL>
+template <typename T, typename RT, int NV, int LPR, int TAIL>
 static void launch_q8_norm_fwd(const Q8FwdArgs& a, bool is_rms, hipStream_t s) {
   const dim3 grid{unsigned((a.rows + Q8Group<LPR>::kRows - 1) / Q8Group<LPR>::kRows)}, block{LPR ? 256u : unsigned(a.threads)};
   // four workgroups of 256 threads to a compute unit where a 16-bit residual comes along: more of them read and write more rows
@@ -520,7 +533,7 @@ static void launch_q8_norm_fwd(const Q8FwdArgs& a, bool is_rms, hipStream_t s) {
   }
   profile_after(s);
 }
-template <typename T, typename RT, int NV, int LPR, int MAXT, bool TAIL>
+template <typename T, typename RT, int NV, int LPR, int MAXT, int TAIL>
 static void launch_q8_norm_bwd(const Q8BwdArgs& a, bool is_rms, hipStream_t s) {
   const dim3 grid{unsigned(a.grid)}, block{LPR ? 256u : unsigned(a.threads)};
   const size_t lds = LPR ? size_t(Q8Group<LPR>::kRows) * a.blocks * kQ8Block * sizeof(float) : 0;
@@ -539,22 +552,23 @@ static void launch_q8_norm_bwd(const Q8BwdArgs& a, bool is_rms, hipStream_t s) {
 template <typename T, typename RT, int WHAT, typename A>
 static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStream_t s) {
   const bool tail = a.cols != shape.nv * shape.lanes * q8_vec<T, RT>();   // a lane's vector may lie outside the row
+#define HK_Q8_TAIL(NV, LPR, TAIL)                                                                    \
+  do {                                                                                               \
+    constexpr int kMost = LPR ? 256 : 512;                                                           \
+    if constexpr (WHAT == 0) launch_q8_norm_fwd<T, RT, NV, LPR, TAIL>(a, is_rms, s);                 \
+    else if (LPR == 0 && a.threads > kMost) launch_q8_norm_bwd<T, RT, NV, LPR, LPR ? kMost : 1024, TAIL>(a, is_rms, s); \
+    else launch_q8_norm_bwd<T, RT, NV, LPR, kMost, TAIL>(a, is_rms, s);                              \
+  } while (0)
 #define HK_Q8(NV, LPR)                                                                               \
   do {                                                                                               \
-    if constexpr (WHAT == 0) {                                                                       \
-      if (tail) launch_q8_norm_fwd<T, RT, NV, LPR, true>(a, is_rms, s);                              \
-      else launch_q8_norm_fwd<T, RT, NV, LPR, false>(a, is_rms, s);                                  \
-    } else {                                                                                         \
-      constexpr int kMost = LPR ? 256 : 512;                                                         \
-      if (LPR == 0 && a.threads > kMost) {                                                           \
-        if (tail) launch_q8_norm_bwd<T, RT, NV, LPR, LPR ? kMost : 1024, true>(a, is_rms, s);        \
-        else launch_q8_norm_bwd<T, RT, NV, LPR, LPR ? kMost : 1024, false>(a, is_rms, s);            \
-      } else if (tail) launch_q8_norm_bwd<T, RT, NV, LPR, kMost, true>(a, is_rms, s);                \
-      else launch_q8_norm_bwd<T, RT, NV, LPR, kMost, false>(a, is_rms, s);                           \
-    }                                                                                                \
+    if (tail) HK_Q8_TAIL(NV, LPR, kTail);                                                            \
+    else HK_Q8_TAIL(NV, LPR, kWhole);                                                                \
   } while (0)
   switch (shape.lanes) {
-    case 8: HK_Q8(1, 8); break;
+    case 8:
+      if (a.cols < q8_vec<T, RT>()) HK_Q8_TAIL(1, 8, kShort);
+      else HK_Q8(1, 8);
+      break;
     case 16: HK_Q8(1, 16); break;
     case 32: HK_Q8(1, 32); break;
     case 64:
@@ -576,6 +590,7 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
       }
   }
 #undef HK_Q8
+#undef HK_Q8_TAIL
   return launch_check(WHAT == 0 ? "q8_norm_fwd_kernel" : "q8_norm_bwd_kernel");
 }
 
