@@ -7,6 +7,8 @@
 
 #include "hk_common.h"
 
+#include <type_traits>
+
 namespace hk {
 
 constexpr int kQ8Block = 32;
@@ -17,18 +19,24 @@ inline int64_t q8_blocks(int64_t cols) { return (cols + kQ8Block - 1) / kQ8Block
 // fp32 beside bf16 rows, read as two 16-byte loads 32 bytes apart: the forward norm of 32768 x 4096 in 430 us instead of
 // 284).  kTail: the row may end before or inside a vector, which is then loaded as the row's last N elements and moved down, so that every load is a whole vector
 // inside the row and none sits in a branch; kWhole: every vector lies inside; kShort: the row may be shorter than a load, a
-// variant of its own, since the branch for it makes the compiler wait for loads that are under way.  raw is the load, floats()
-// what comes of it.
+// variant of its own, since the branch for it makes the compiler wait for loads that are under way.  kOdd: as kTail, and rows of
+// 16-bit elements may begin on an odd element, where a load of 16 bytes takes a multiple of its time: those load from one
+// column on, and the first column of a lane's vector comes from the lane before it, or for the wavefront's first lane (of a
+// row) from a load of its own.  raw is the load, floats() what comes of it.
 typedef u32x2 u32x2_on2 __attribute__((aligned(2)));
-constexpr int kWhole = 0, kTail = 1, kShort = 2;
+constexpr int kWhole = 0, kTail = 1, kShort = 2, kOdd = 3;
 template <typename R, int N, int TAIL>
 struct RowVec {
   static constexpr int kWords = N * int(sizeof(R)) / 4;
   static_assert(kWords == 4 || kWords == 2, "one load of 16 or 8 bytes");
   u32x4 raw;
+  static constexpr bool kOddRows = TAIL == kOdd && sizeof(R) == 2;
+  struct Nothing {};
+  typename std::conditional<kOddRows, uint32_t, Nothing>::type first;   // kOddRows: the wavefront's first element
+  typename std::conditional<kOddRows, bool, Nothing>::type odd;
   // row: any element boundary; one of cols elements, cols >= 1
   template <bool KEEP = false>   // KEEP: read by many workgroups
-  __device__ __forceinline__ void load(const R* row, int c, int cols) {
+  __device__ __forceinline__ void load(const R* row, int c, int cols, [[maybe_unused]] int lane_in_row = 0) {
     if (TAIL == kShort && cols < N) {   // uniform
       float f[8] = {};
       if (c == 0) {
@@ -39,8 +47,14 @@ struct RowVec {
       raw = VecIO<R>::pack(f);
       return;
     }
+    int from = c;
+    if constexpr (kOddRows) {
+      odd = (reinterpret_cast<uintptr_t>(row) & 2u) != 0;
+      from += odd ? 1 : 0;
+      first = *reinterpret_cast<const uint16_t*>(row + min(c - (lane_in_row & 63) * N, cols - 1));
+    }
     // (a scalar base and 32 bits of offset)
-    const R* p = reinterpret_cast<const R*>(reinterpret_cast<const char*>(row) + uint32_t(TAIL ? min(c, cols - N) : c) * uint32_t(sizeof(R)));
+    const R* p = reinterpret_cast<const R*>(reinterpret_cast<const char*>(row) + uint32_t(TAIL ? min(from, cols - N) : c) * uint32_t(sizeof(R)));
     if constexpr (kWords == 4) {
       if constexpr (KEEP) raw = ld16_any_keep<R>(p);
       else raw = ld16_any<R>(p);
@@ -52,8 +66,16 @@ struct RowVec {
     }
   }
   // full (uniform): every lane's vector lies inside the row
-  __device__ __forceinline__ void floats(float* f, int c, int cols, bool full = false) const {
+  __device__ __forceinline__ void floats(float* f, int c, int cols, bool full = false, [[maybe_unused]] int lane_in_row = 0) const {
     u32x4 r = raw;
+    if constexpr (kOddRows) {
+      constexpr int kWaveShr1 = 0x138;
+      uint32_t before = uint32_t(__builtin_amdgcn_update_dpp(0, int(raw[kWords - 1]), kWaveShr1, 0xf, 0xf, false));
+      before = (lane_in_row & 63) == 0 ? first << 16 : before;
+      const bool shifted = odd && c < cols - N;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) r[k] = shifted ? __builtin_amdgcn_alignbit(raw[k], k ? raw[k - 1] : before, 16) : raw[k];
+    }
     if constexpr (TAIL) {
       if (!full && (TAIL != kShort || cols >= N)) {   // uniform
         const int bits = (c - min(c, cols - N)) * int(sizeof(R)) * 8;

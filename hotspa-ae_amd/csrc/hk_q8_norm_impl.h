@@ -39,7 +39,7 @@ struct Q8Group {
 // reduction: it may lie over the residual, and every lane has read its part of the row by then.  The 8 bits go out before it:
 // they need no statistics, and nothing waits for them.  Bound by memory (32768 x 4096 bf16, us here / what the bytes take:
 // RMSNorm 102 / 99, with a bf16 residual 182 / 178, with one in fp32 274 / 257; LayerNorm of 16384 x 5120 68 / 62); odd widths
-// pay for loads and stores that begin on any element (LayerNorm of 9000 rows bf16: 29.5 at 3584 columns, 34.5 at 3579; 30.0 at
+// pay for loads and stores that begin on any element (LayerNorm of 9000 rows bf16: 29.5 at 3584 columns, 33.0 at 3579; 30.0 at
 // 3579 with the rows on 16-byte boundaries).
 template <typename T, typename RT, int NV, int LPR, bool HAS_RES, bool IS_RMS, int TAIL>
 __global__ __launch_bounds__(LPR ? 256 : 1024)
@@ -59,7 +59,7 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
 
   const T* gp = static_cast<const T*>(a.gamma);
   const T* bp = static_cast<const T*>(a.beta);
-  RowVec<T, VEC, TAIL> g[NV], b[NV];
+  RowVec<T, VEC, TAIL == kOdd ? kTail : TAIL> g[NV], b[NV];
   float v[NV][VEC];
   {
     RowVec<T, VEC, TAIL> x[NV];
@@ -68,15 +68,15 @@ void q8_norm_fwd_kernel(Q8FwdArgs a) {
     const RT* rr = HAS_RES ? static_cast<const RT*>(a.residual) + row * a.res_pitch : nullptr;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      x[i].load(xr, column(i), cols);
-      if constexpr (HAS_RES) r[i].load(rr, column(i), cols);
+      x[i].load(xr, column(i), cols, t);
+      if constexpr (HAS_RES) r[i].load(rr, column(i), cols, t);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      x[i].floats(v[i], column(i), cols, full(i));
+      x[i].floats(v[i], column(i), cols, full(i), t);
       if constexpr (HAS_RES) {
         float f[VEC];
-        r[i].floats(f, column(i), cols, full(i));
+        r[i].floats(f, column(i), cols, full(i), t);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[i][j] += f[j];
       }
@@ -211,7 +211,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   const T* gp = static_cast<const T*>(a.gamma);
   // gamma as fp32, packed where that is more registers than there are
   constexpr bool kPacked = NE > 16 && sizeof(T) == 2;
-  RowVec<T, VEC, TAIL> gm[NV];
+  RowVec<T, VEC, TAIL == kOdd ? kTail : TAIL> gm[NV];
   [[maybe_unused]] float gf[kPacked ? 1 : NE];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -249,10 +249,10 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = uint32_t(TAIL ? min(column(i), pitch - VEC) : column(i));
-      next.dz[i].load(dr, column(i), cols);
+      next.dz[i].load(dr, column(i), cols, t);
       next.q[i] = __builtin_nontemporal_load(reinterpret_cast<const typename Words::type*>(qr + c));
       next.e[i] = sr[c / kQ8Block];
-      if constexpr (EXTRA) next.up[i].load(ur, column(i), cols);
+      if constexpr (EXTRA) next.up[i].load(ur, column(i), cols, t);
     }
   };
   const int64_t stride = int64_t(a.grid) * Group::kRows;
@@ -271,10 +271,12 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
     float step_of[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      next.dz[i].floats(&u[i * VEC], column(i), cols, full(i));
+      next.dz[i].floats(&u[i * VEC], column(i), cols, full(i), t);
       Words::numbers(next.q[i], &x[i * VEC]);
       step_of[i] = rs * q8_step(next.e[i]);   // (a power of two: exact)
       if constexpr (EXTRA) up[i] = next.up[i];
+      // (here before the reduction: the gradient may be written over it, and a vector may reach into another wavefront's columns)
+      if constexpr (EXTRA && TAIL != kWhole && LPR == 0) asm volatile("" ::"v"(up[i].raw));
     }
     issue(row + stride);
     SumTuple<KS> s = SumTuple<KS>::identity();
@@ -311,7 +313,7 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
       for (int i = 0; i < NV; ++i) {
         float o[VEC];
         [[maybe_unused]] float add[VEC];
-        if constexpr (EXTRA) up[i].floats(add, column(i), cols, full(i));
+        if constexpr (EXTRA) up[i].floats(add, column(i), cols, full(i), t);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int e = i * VEC + j;
@@ -548,10 +550,22 @@ static void launch_q8_norm_bwd(const Q8BwdArgs& a, bool is_rms, hipStream_t s) {
   profile_after(s);
 }
 
+// whether rows begin on odd elements of 16 bits
+static inline bool odd_rows(const void* rows, int64_t pitch) {
+  return rows && ((pitch & 1) || (reinterpret_cast<uintptr_t>(rows) & 2u));
+}
 // WHAT: 0 forward, 1 backward
 template <typename T, typename RT, int WHAT, typename A>
 static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStream_t s) {
   const bool tail = a.cols != shape.nv * shape.lanes * q8_vec<T, RT>();   // a lane's vector may lie outside the row
+  // rows that begin on odd elements of 16 bits, where a workgroup holds a row (us as any row / so: LayerNorm of 9000 x 3579 bf16,
+  // forward 34.5 / 33.0, with a residual 63.3 / 58.2, backward with an upstream gradient 69.6 / 61.2; not where a wavefront holds
+  // it, 8192 x 1021 fp16 forward 9.7 / 10.4, nor at 8-byte loads beside fp32, 9000 x 3579 72.4 / 73.3)
+  bool odd = false;
+  if constexpr (q8_vec<T, RT>() == 8) {
+    if constexpr (WHAT == 0) odd = odd_rows(a.x0, a.x0_pitch) || odd_rows(a.residual, a.res_pitch);
+    else odd = odd_rows(a.dz, a.dz_pitch) || odd_rows(a.dx_in, a.dxin_pitch);
+  }
 #define HK_Q8_TAIL(NV, LPR, TAIL)                                                                    \
   do {                                                                                               \
     constexpr int kMost = LPR ? 256 : 512;                                                           \
@@ -561,7 +575,9 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
   } while (0)
 #define HK_Q8(NV, LPR)                                                                               \
   do {                                                                                               \
-    if (tail) HK_Q8_TAIL(NV, LPR, kTail);                                                            \
+    if (odd && LPR == 0) {                                                                           \
+      if constexpr (LPR == 0 && q8_vec<T, RT>() == 8) HK_Q8_TAIL(NV, LPR, kOdd);                     \
+    } else if (tail) HK_Q8_TAIL(NV, LPR, kTail);                                                            \
     else HK_Q8_TAIL(NV, LPR, kWhole);                                                                \
   } while (0)
   switch (shape.lanes) {

@@ -385,6 +385,46 @@ def test_pitched_rows(hk, cuda, cols):
             assert bool((base[:, :first + 1] == 3).all()) and bool((base[:, first + 1 + cols:] == 3).all())
 
 
+@pytest.mark.parametrize("dtype,rtype", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "fp32"), ("fp16", "")])
+@pytest.mark.parametrize("cols", [2057, 2560, 3579, 4095, 4096, 8200, 9001, 17001])
+def test_rows_on_odd_elements(hk, cuda, dtype, rtype, cols):
+    """Rows of 16-bit elements that begin on odd ones, between columns of NaN, give what the same rows on 16-byte boundaries
+    give, bit by bit; also where the gradients are written over what they are made of."""
+    import torch
+    gen = torch.Generator(device=cuda).manual_seed(cols)
+    for rows, places in ((37, ((1, 4, 1, 2), (0, 1, 3, 0))), (1300, ((1, 1, 3, 8),))):
+        whole = (cols + 7) // 8 * 8 + 16
+        data = [torch.randn((rows, cols), generator=gen, device=cuda).to(_dt(t)) if t else None for t in (dtype, rtype, dtype, rtype)]
+        gamma = (torch.rand(cols, generator=gen, device=cuda) + 0.5).to(_dt(dtype))
+        sides = []
+        for place in ((8, 8, 8, 8),) + places:
+            def rows_at(first, value, t):
+                if value is None and t is None:
+                    return None
+                width = whole if place[0] == 8 else whole + 1 + place[3] % 2
+                out = torch.full((rows, width), math.nan, device=cuda, dtype=_dt(t) if t else value.dtype)[:, first:first + cols]
+                if value is not None:
+                    out.copy_(value)
+                return out
+            x0, res, dz, up = (rows_at(f, v, None) for f, v in zip(place, data))
+            z, dx = rows_at(place[2], None, dtype), rows_at(place[1], None, dtype)
+            s = rows_at(place[0], None, rtype) if rtype else None
+            q, scale = hk.q8_empty(rows, cols, cuda)
+            mu, rs, dg = torch.empty(rows, device=cuda), torch.empty(rows, device=cuda), torch.empty_like(gamma)
+            hk.add_ln_q8_fwd(x0, res, gamma, None, z, s, q, scale, mu, rs, EPS, True)
+            hk.add_ln_q8_bwd(dz, up, q, scale, mu, rs, gamma, dx, None, dg, None, True)
+            kept = [t.clone() for t in (z, q, scale, mu, rs, dx, dg)] + ([s.clone()] if rtype else [])
+            if rtype and rows > 1024:
+                hk.add_ln_q8_bwd(dz, up, q, scale, mu, rs, gamma, dz, up, dg, None, True)
+                assert torch.equal(dz, dx) and torch.equal(up, dx if rtype == dtype else up) and torch.equal(dg, kept[6])
+            if rtype:
+                hk.add_ln_q8_fwd(x0, res, gamma, None, z, res, q, scale, mu, rs, EPS, True)
+                assert torch.equal(res, s) and torch.equal(z, kept[0])
+            sides.append(kept)
+        for other in sides[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(sides[0], other))
+
+
 def test_rows_with_nan_stay_by_themselves(hk, cuda):
     """A row that holds a NaN gives NaN in its own row; the other rows' results are as without it."""
     import torch
