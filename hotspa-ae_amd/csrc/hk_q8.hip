@@ -35,7 +35,8 @@ __device__ __forceinline__ Q8Place q8_place(const Q8FlatArgs& a, uint32_t v, int
   return {row, int(v - row * a.row_vecs) * vec};
 }
 
-// Packing and unpacking, two vectors a thread in workgroups of 256; bound by memory.  One vector and 64 threads / so, us, of what
+// Packing and unpacking, two vectors a thread in workgroups of 256; bound by memory.  One vector and 64 threads / so, us (one set
+// of arrays, in part from a cache), of what
 // the bytes take: packing 32768 x 4096 bf16 67 / 58.6 of 59.8, 14549 x 3579 fp32 45 / 38 of 38.5; unpacking the same 62.5 / 64
 // and 52 / 44.
 template <typename T, int TAIL, int U>
