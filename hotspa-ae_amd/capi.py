@@ -560,7 +560,7 @@ def token_logprob_fwd(logits, tokens, logprob, entropy, lse, top_logprob, top_to
     if ref is None or not (n.values(rows, 4, dev, tokens) and n.values(rows, 6, dev, logprob, entropy, lse) and
                            n.values(rows * top, 6, dev, top_logprob) and n.values(rows * top, 4, dev, top_token)):
         import torch
-        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        rows = logits.numel() // logits.shape[-1] if logits.dim() and logits.numel() else 0
         _refuse("token_logprob_fwd", logits, rows, [
             ("tokens", tokens, rows, torch.int64), ("logprob", logprob, rows, torch.float32),
             ("entropy", entropy, rows, torch.float32), ("lse", lse, rows, torch.float32),
@@ -583,7 +583,7 @@ def token_logprob_bwd(logits, tokens, lse, entropy, grad_logprob, grad_entropy, 
         out = n.row_pitches(rows, cols, code, dev, dlogits)
     if out is None or not (n.values(rows, 4, dev, tokens) and n.values(rows, 6, dev, lse, entropy, grad_logprob, grad_entropy)):
         import torch
-        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        rows = logits.numel() // logits.shape[-1] if logits.dim() and logits.numel() else 0
         _refuse("token_logprob_bwd", logits, rows, [
             ("tokens", tokens, rows, torch.int64), ("lse", lse, rows, torch.float32), ("entropy", entropy, rows, torch.float32),
             ("grad_logprob", grad_logprob, rows, torch.float32), ("grad_entropy", grad_entropy, rows, torch.float32)],
@@ -604,7 +604,7 @@ def vocab_parallel_logprob_stats(logits, tokens, stats, top_value, top_token, vo
     if ref is None or not (n.values(rows, 4, dev, tokens) and n.values(4 * rows, 6, dev, stats) and
                            n.values(rows * top, 6, dev, top_value) and n.values(rows * top, 4, dev, top_token)):
         import torch
-        rows = logits.numel() // logits.shape[-1] if logits.numel() else 0
+        rows = logits.numel() // logits.shape[-1] if logits.dim() and logits.numel() else 0
         _refuse("vocab_parallel_logprob_stats", logits, rows, [
             ("tokens", tokens, rows, torch.int64), ("stats", stats, 4 * rows, torch.float32),
             ("top_value", top_value, rows * top, torch.float32), ("top_token", top_token, rows * top, torch.int64)])
@@ -669,8 +669,9 @@ def q8_pack(x, q, scale, stream=None):
         rows, cols, pitch, code, dev = ref
         blocks = rows * ((cols + 31) >> 5)
     if ref is None or not (n.values(blocks * 32, 1, dev, q) and n.values(blocks, 0, dev, scale)):
-        rows = x.numel() // x.shape[-1] if x.numel() else 0
-        _refuse("q8_pack", x, rows, _q8_values(q, scale, rows, x.shape[-1]))
+        cols = x.shape[-1] if x.dim() else 0
+        rows = x.numel() // cols if cols else 0
+        _refuse("q8_pack", x, rows, _q8_values(q, scale, rows, cols))
     check(n.hk_q8_pack(code, x, pitch, q, scale, rows, cols, stream))
 
 
@@ -681,8 +682,9 @@ def q8_unpack(q, scale, out, stream=None):
         rows, cols, pitch, code, dev = ref
         blocks = rows * ((cols + 31) >> 5)
     if ref is None or not (n.values(blocks * 32, 1, dev, q) and n.values(blocks, 0, dev, scale)):
-        rows = out.numel() // out.shape[-1] if out.numel() else 0
-        _refuse("q8_unpack", out, rows, _q8_values(q, scale, rows, out.shape[-1]))
+        cols = out.shape[-1] if out.dim() else 0
+        rows = out.numel() // cols if cols else 0
+        _refuse("q8_unpack", out, rows, _q8_values(q, scale, rows, cols))
     check(n.hk_q8_unpack(code, q, scale, out, pitch, rows, cols, stream))
 
 

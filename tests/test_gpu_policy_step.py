@@ -220,5 +220,14 @@ def test_operator_layer_refusals(hk, cuda):
         hk.add_ln_q8_fwd(x, x, None, None, x, x.half(), q, scale, v, v, EPS, True)
     with pytest.raises(hk.HkError, match="shape"):
         hk.token_logprob_bwd(x, tok, v, None, v, None, x[:, :32], IGN)
+    one = torch.zeros((), device=cuda)
+    for call in (lambda: hk.token_logprob_fwd(one, tok, v, None, None, None, None, IGN),
+                 lambda: hk.token_logprob_bwd(one, tok, v, None, v, None, one, IGN),
+                 lambda: hk.vocab_parallel_logprob_stats(one, tok, torch.zeros(4, 1, device=cuda), None, None, 0, IGN),
+                 lambda: hk.q8_pack(one, q, scale), lambda: hk.q8_unpack(q, scale, one),
+                 lambda: hk.add_ln_q8_fwd(one, None, None, None, one, None, q, scale, v, v, EPS, True),
+                 lambda: hk.add_ln_q8_out(q, scale, v, v, None, None, one, True)):
+        with pytest.raises(hk.HkError, match="scalar"):
+            call()
     with pytest.raises(hk.HkError, match="unit-stride"):
         hk.token_logprob_fwd(torch.zeros(64, 4, device=cuda).t(), tok, v, None, None, None, None, IGN)
