@@ -566,7 +566,9 @@ def token_logprob_fwd(logits, tokens, logprob, entropy, lse, top_logprob, top_to
             ("entropy", entropy, rows, torch.float32), ("lse", lse, rows, torch.float32),
             ("top_logprob", top_logprob, rows * top, torch.float32), ("top_token", top_token, rows * top, torch.int64)])
     if workspace is None and rows:
-        workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top), logits.device)
+        need = n.token_logprob_workspace(code, rows, cols, top)
+        if need != 0:
+            workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top) if need is None else need, logits.device)
     check(n.hk_token_logprob_fwd(code, logits, pitch, tokens, logprob, entropy, lse, top_logprob, top_token, top, rows, cols,
                                  ignored_index, workspace, _size(workspace), stream))
     return workspace
@@ -609,7 +611,9 @@ def vocab_parallel_logprob_stats(logits, tokens, stats, top_value, top_token, vo
             ("tokens", tokens, rows, torch.int64), ("stats", stats, 4 * rows, torch.float32),
             ("top_value", top_value, rows * top, torch.float32), ("top_token", top_token, rows * top, torch.int64)])
     if workspace is None and rows:
-        workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top), logits.device)
+        need = n.token_logprob_workspace(code, rows, cols, top)
+        if need != 0:
+            workspace = _workspace(token_logprob_workspace_bytes(code, rows, cols, top) if need is None else need, logits.device)
     check(n.hk_vocab_parallel_logprob_stats(code, logits, pitch, tokens, stats, top_value, top_token, top, rows, cols,
                                             vocab_start, ignored_index, workspace, _size(workspace), stream))
     return workspace
@@ -745,7 +749,8 @@ def add_ln_q8_bwd(dz, dx_in, q, scale, mu, rsigma, gamma, dx0, dresidual, dgamma
     rows, cols, code, rcode, zp, (xp,), (ip, rp) = _q8_norm(n, "add_ln_q8_bwd", dz, q, scale, (mu, rsigma),
                                                             (gamma, dgamma, dbeta), (dx0,), (dx_in, dresidual))
     if workspace is None and (dgamma is not None or dbeta is not None):
-        workspace = _workspace(add_ln_q8_bwd_workspace_bytes(rows, cols), dz.device)
+        need = n.add_ln_q8_bwd_workspace(rows, cols)
+        workspace = _workspace(add_ln_q8_bwd_workspace_bytes(rows, cols) if need is None else need, dz.device)
     check(n.hk_add_ln_q8_bwd(code, rcode, dz, zp, dx_in, ip, q, scale, mu, rsigma, gamma, dx0, xp, dresidual, rp, dgamma, dbeta,
                              rows, cols, int(is_rms), workspace, _size(workspace), stream))
     return workspace

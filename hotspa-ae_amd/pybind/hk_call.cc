@@ -437,6 +437,27 @@ PyObject* values(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+#ifndef HT_CALL
+// bytes of scratch that a call asks for, None where it refuses its sizes: token_logprob_workspace(code, rows, cols, top),
+// add_ln_q8_bwd_workspace(rows, cols)
+PyObject* token_logprob_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  int64_t v[4];
+  size_t bytes = 0;
+  if (n != 4) return answer_none();
+  for (int i = 0; i < 4; ++i)
+    if (!to_i64(args[i], &v[i])) return answer_none();
+  if (hk_token_logprob_workspace_bytes(int(v[0]), v[1], v[2], v[3], &bytes) != HK_OK) return answer_none();
+  return PyLong_FromSize_t(bytes);
+}
+PyObject* add_ln_q8_bwd_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  int64_t rows, cols;
+  size_t bytes = 0;
+  if (n != 2 || !to_i64(args[0], &rows) || !to_i64(args[1], &cols)) return answer_none();
+  if (hk_add_ln_q8_bwd_workspace_bytes(rows, cols, &bytes) != HK_OK) return answer_none();
+  return PyLong_FromSize_t(bytes);
+}
+#endif
+
 PyObject* setup(PyObject*, PyObject* args) {
   return PyArg_ParseTuple(args, "OOOO", &g_dtype_codes, &g_current_stream, &g_get_device, &g_raw_stream)
              ? (Py_INCREF(g_dtype_codes), Py_INCREF(g_current_stream), Py_INCREF(g_get_device), Py_INCREF(g_raw_stream),
@@ -454,6 +475,8 @@ PyMethodDef methods[] = {
     {"row_pitches", (PyCFunction)(void (*)())row_pitches, METH_FASTCALL, nullptr},
     {"values", (PyCFunction)(void (*)())values, METH_FASTCALL, nullptr},
 #ifndef HT_CALL
+    {"token_logprob_workspace", (PyCFunction)(void (*)())token_logprob_workspace, METH_FASTCALL, nullptr},
+    {"add_ln_q8_bwd_workspace", (PyCFunction)(void (*)())add_ln_q8_bwd_workspace, METH_FASTCALL, nullptr},
     ENTRY(dropout_fwd_ex), ENTRY(dropout_bwd_ex), ENTRY(hk_batch_norm_bwd), ENTRY(hk_batch_norm_fwd),
     ENTRY(hk_binary_const), ENTRY(hk_dropout_add_ln_bwd_pitched), ENTRY(hk_dropout_add_ln_fwd_pitched),
     ENTRY(hk_layer_norm_bwd_pitched), ENTRY(hk_layer_norm_fwd_pitched), ENTRY(hk_reduce), ENTRY(hk_sce_dense_bwd),
