@@ -219,7 +219,7 @@ struct Q8BwdArgs {
   float inv_cols;
   int rows, cols, blocks, grid;
   uint16_t threads;
-  bool few;                 // part_dgamma / part_dbeta are then dgamma / dbeta themselves
+  uint8_t few;              // 1, 2: without partial rows, in one launch or two; part_dgamma / part_dbeta are then dgamma / dbeta
 };
 
 constexpr int kQ8MaxCols = 32768;

@@ -249,13 +249,15 @@ Q8Shape q8_fwd_shape(int64_t cols, int vec) {
 }
 // One vector a thread where 1024 threads hold the row in 16-byte vectors of 16-bit elements: twice the wavefronts, whose
 // loads and reductions hide one another (LayerNorm of 16384 x 5120 bf16, 320 threads x 2 / 640 x 1: 88.4 / 79.9 us; RMSNorm of
-// 32768 x 4096 with an upstream gradient, 256 x 2 / 512 x 1: 200 / 196).
+// 32768 x 4096 with an upstream gradient, 256 x 2 / 512 x 1: 200 / 196).  Of more, up to 1024 threads before a thread takes twice
+// as many columns (RMSNorm of 4096 x 10240 bf16 with an upstream gradient, 320 x 4 / 640 x 2: 100 / 79, without 47 / 44, of 12289
+// 277 / 174 and 96 / 71; LayerNorm without one 69 / 77).
 Q8Shape q8_bwd_shape(int64_t cols, int vec) {
   const int64_t n = q8_blocks(cols) * (kQ8Block / vec);
   Q8Shape s;
   if (q8_wave_shape(n, &s)) return s;
   if (vec == 8 && n <= 1024) return {int((n + 63) / 64 * 64), 1};
-  return q8_group_shape(n, vec == 4 ? 8 : 4, 512);
+  return q8_group_shape(n, vec == 4 ? 8 : 4, 1024);
 }
 // As many workgroups as fill a compute unit to 1024 threads; to 512 where an upstream gradient comes in and the rows' loads are
 // half as many again (RMSNorm of 32768 x 4096 bf16, one / two / four workgroups of 512 threads to a compute unit: with it 196 /
@@ -273,6 +275,15 @@ int q8_bwd_grid(int64_t rows, const Q8Shape& shape, bool extra) {
 // rows and a fold: LayerNorm of 768 x 4096 bf16 6.4 / 17.4, 1024 8.0 / 18.5, of 1024 x 1024 6.9 / 6.8; with an upstream gradient in
 // fp32 768 x 4096 11.6 / 12.7, 1024 16.1 / 14.9).
 static int64_t q8_few_rows(bool extra) { return extra ? 768 : 1024; }
+// Rows whose backward is two launches, the column sums from the rows themselves, then dx: where a thread would keep the sums of
+// more than 16 columns, which spill, or of 16 beside an upstream gradient, in the half of the registers that more than 512
+// threads leave (persistent / two launches, us, 4096 rows: 20480 bf16 508 / 169, with an upstream gradient 785 / 208; 12288
+// fp32 with one 224 / 207, bf16 with one in fp32 203 / 164, LayerNorm bf16 with one 130 / 119; but RMSNorm 89 / 117 and without
+// one 52 / 96).
+static bool q8_wide(const Q8Shape& shape, int vec, bool extra, bool is_rms) {
+  const int columns = shape.nv * vec;
+  return shape.lanes > kWave && (columns > 16 || (columns == 16 && shape.lanes > 512 && extra && (vec == 4 || !is_rms)));
+}
 // nothing that is written may lie over what is read there
 static bool q8_apart(const Q8BwdArgs& a, const void* dgamma, const void* dbeta, size_t es, size_t rs) {
   const int64_t rows = a.rows, cols = a.cols;
@@ -406,7 +417,8 @@ int hk_add_ln_q8_bwd(int itype, int rtype, const void* dz, int64_t dz_pitch, con
              (!dresidual || dresidual_pitch >= cols), HK_ERR_INVALID, "hk_add_ln_q8_bwd: row pitch below the columns");
   HK_REQUIRE((reinterpret_cast<uintptr_t>(q) & 7u) == 0, HK_ERR_INVALID, "hk_add_ln_q8_bwd: q must lie on an 8-byte boundary");
   if (!dx_in && !dresidual) rtype = itype;
-  const Q8Shape shape = q8_bwd_shape(cols, rtype == HK_FLOAT32 ? 4 : 8);
+  const int vec = rtype == HK_FLOAT32 ? 4 : 8;
+  const Q8Shape shape = q8_bwd_shape(cols, vec);
   Q8BwdArgs a{};
   a.blocks = int(q8_blocks(cols));
   a.grid = q8_bwd_grid(rows, shape, dx_in != nullptr);
@@ -421,8 +433,9 @@ int hk_add_ln_q8_bwd(int itype, int rtype, const void* dz, int64_t dz_pitch, con
   a.dz = dz; a.dz_pitch = dz_pitch; a.dx_in = dx_in; a.dxin_pitch = dx_in_pitch; a.gamma = gamma; a.q = q; a.scale = scale;
   a.mu = mu; a.rs = rsigma; a.dx0 = dx0; a.dx_pitch = dx0_pitch; a.dres = dresidual; a.dres_pitch = dresidual_pitch;
   a.rows = int(rows); a.cols = int(cols); a.inv_cols = 1.0f / float(cols); a.threads = uint16_t(shape.lanes);
-  a.few = rows <= q8_few_rows(dx_in != nullptr) && shape.lanes >= kWave && shape.lanes <= kSmallThreads && shape.nv <= 4 && (dgamma || dbeta) &&
+  a.few = rows <= q8_few_rows(dx_in != nullptr) && shape.lanes >= kWave && shape.lanes <= kSmallThreads && (dgamma || dbeta) &&
           q8_apart(a, dgamma, dbeta, dtype_size(itype), dtype_size(rtype));
+  if (!a.few && q8_wide(shape, vec, dx_in != nullptr, is_rms_norm != 0)) a.few = 2;
 #define HK_CALL_BWD(T) q8_norm_bwd_typed<T>(a, rtype, is_rms_norm != 0, shape, dgamma, dbeta, s)
   return HK_Q8_TYPED(itype, HK_CALL_BWD);
 #undef HK_CALL_BWD

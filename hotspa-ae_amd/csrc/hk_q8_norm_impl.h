@@ -363,10 +363,10 @@ void q8_norm_bwd_kernel(Q8BwdArgs a) {
   if constexpr (!IS_RMS) leave(a.part_dbeta, db);
 }
 
-// The whole backward of few rows in one launch: the first `sums` workgroups form the column sums of 8 vectors of columns each,
+// The whole backward without partial rows, of few rows in one launch (of wide ones in two: the sums, then dx): the first `sums` workgroups form the column sums of 8 vectors of columns each,
 // from all rows, the others dx, rows side by side in a workgroup.  The partial rows that the kernel above would leave are as
 // many bytes as the rows themselves by then (LayerNorm of 512 x 4096 bf16: 16.8 us with them and their fold, 5.2 so).  Only
-// where nothing that is written lies over what is read.
+// where nothing that is written lies over what is read, or in two launches.
 template <typename T, typename RT, int NV, bool EXTRA, bool IS_RMS, int TAIL>
 __global__ __launch_bounds__(kSmallThreads)
 void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
@@ -435,6 +435,9 @@ void q8_norm_bwd_few_kernel(Q8BwdArgs a, int sums) {
     if (gp) rg[i].template load<true>(gp, column(i), cols);   // uniform
     if constexpr (EXTRA) up[i].load(static_cast<const RT*>(a.dx_in) + row * a.dxin_pitch, column(i), cols);
   }
+  if constexpr (EXTRA && TAIL != kWhole)   // as above
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" ::"v"(up[i].raw));
   const float rs = a.rs[row];
   [[maybe_unused]] const float shift = IS_RMS ? 0.f : -rs * a.mu[row];
   float x[NV][VEC], u[NV][VEC];
@@ -483,13 +486,7 @@ static void launch_q8_norm_few(const Q8BwdArgs& a, bool is_rms, dim3 grid, int s
   profile_after(s);
 }
 template <typename T, typename RT>
-static int q8_norm_few(Q8BwdArgs a, bool is_rms, const Q8Shape& shape, void* dgamma, void* dbeta, hipStream_t s) {
-  constexpr int VEC = q8_vec<T, RT>();
-  a.part_dgamma = static_cast<float*>(dgamma);
-  a.part_dbeta = static_cast<float*>(dbeta);
-  const bool tail = a.cols != shape.nv * shape.lanes * VEC;
-  const int sums = (a.blocks * kQ8Block + 8 * VEC - 1) / (8 * VEC), rpb = kSmallThreads / shape.lanes;
-  const dim3 grid{unsigned(sums + (a.rows + rpb - 1) / rpb)};
+static int launch_q8_norm_few_shape(const Q8BwdArgs& a, bool is_rms, const Q8Shape& shape, bool tail, dim3 grid, int sums, hipStream_t s) {
 #define HK_Q8_FEW(NV)                                                                                                \
   do {                                                                                                               \
     if (a.dx_in) {                                                                                                   \
@@ -503,10 +500,44 @@ static int q8_norm_few(Q8BwdArgs a, bool is_rms, const Q8Shape& shape, void* dga
   switch (shape.nv) {
     case 1: HK_Q8_FEW(1); break;
     case 2: HK_Q8_FEW(2); break;
-    default: HK_Q8_FEW(4); break;
+    case 4: HK_Q8_FEW(4); break;
+    default:
+      if constexpr (q8_vec<T, RT>() == 4) HK_Q8_FEW(8);
+      break;
   }
 #undef HK_Q8_FEW
   return launch_check("q8_norm_bwd_few_kernel");
+}
+template <typename T, typename RT>
+static int q8_norm_few(Q8BwdArgs a, bool is_rms, const Q8Shape& shape, void* dgamma, void* dbeta, hipStream_t s) {
+  constexpr int VEC = q8_vec<T, RT>();
+  a.part_dgamma = static_cast<float*>(dgamma);
+  a.part_dbeta = static_cast<float*>(dbeta);
+  const bool tail = a.cols != shape.nv * shape.lanes * VEC;
+  const int strips = (a.blocks * kQ8Block + 8 * VEC - 1) / (8 * VEC), rpb = kSmallThreads / shape.lanes;
+  if (a.few == 2) {   // the sums first: dx may lie over what they are made of
+    if (dgamma || dbeta) {
+      const int rc = launch_q8_norm_few_shape<T, RT>(a, is_rms, shape, tail, dim3(unsigned(strips)), strips, s);
+      if (rc != HK_OK) return rc;
+    }
+    const int64_t at_once = rows_of_a_launch(kSmallThreads) * rpb;
+    for (int64_t r = 0; r < a.rows; r += at_once) {
+      Q8BwdArgs b = a;
+      b.rows = int(std::min<int64_t>(at_once, a.rows - r));
+      b.dz = static_cast<const T*>(a.dz) + r * a.dz_pitch;
+      b.dx0 = static_cast<T*>(a.dx0) + r * a.dx_pitch;
+      if (b.dx_in) b.dx_in = static_cast<const RT*>(a.dx_in) + r * a.dxin_pitch;
+      if (b.dres) b.dres = static_cast<RT*>(a.dres) + r * a.dres_pitch;
+      b.q = a.q + r * int64_t(a.blocks) * kQ8Block;
+      b.scale = a.scale + r * a.blocks;
+      b.rs = a.rs + r;
+      if (b.mu) b.mu = a.mu + r;
+      const int rc = launch_q8_norm_few_shape<T, RT>(b, is_rms, shape, tail, dim3(unsigned((b.rows + rpb - 1) / rpb)), 0, s);
+      if (rc != HK_OK) return rc;
+    }
+    return HK_OK;
+  }
+  return launch_q8_norm_few_shape<T, RT>(a, is_rms, shape, tail, dim3(unsigned(strips + (a.rows + rpb - 1) / rpb)), strips, s);
 }
 
 // the partial rows folded into dgamma / dbeta (blockIdx.y picks which)
@@ -598,10 +629,11 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
       switch (shape.nv) {
         case 1: HK_Q8(1, 0); break;
         case 2: HK_Q8(2, 0); break;
-        case 4: HK_Q8(4, 0); break;
+        case 4:   // (the backward of wider rows takes another way)
+          if constexpr (WHAT == 0 || q8_vec<T, RT>() == 4) HK_Q8(4, 0);
+          break;
         default:
-          HK_REQUIRE((q8_vec<T, RT>() == 4) && shape.nv == 8, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
-          if constexpr (q8_vec<T, RT>() == 4) HK_Q8(8, 0);
+          if constexpr (WHAT == 0 && q8_vec<T, RT>() == 4) HK_Q8(8, 0);
           break;
       }
   }

@@ -296,6 +296,27 @@ def test_wide_rows(hk, cuda, dtype, cols):
         _check_backward(got, dz, up, *out[2:], gamma, rms, dtype, "fp32", (dtype, cols))
 
 
+@pytest.mark.parametrize("dtype,rtype,cols", [("bf16", "bf16", 12288), ("bf16", "bf16", 17001), ("fp16", "fp32", 9000),
+                                              ("fp32", "fp32", 16384), ("fp16", "", 20000), ("fp32", "fp32", 20011)])
+def test_wide_rows_of_a_batch(hk, cuda, dtype, rtype, cols):
+    """Wide rows, more of them than the one-launch backward takes: against the formula, and over what the gradients are made of."""
+    import torch
+    for rms in (True, False):
+        x0, res, gamma, beta, normal = _norm_inputs(1100, cols, dtype, rtype, cols)
+        out = _forward(hk, x0, res, gamma, None, rms)
+        dz, up = normal(), normal(dt=rtype) if rtype else None
+        got = _backward(hk, dz, up, *out[2:], gamma, rms, bool(rtype))
+        _check_backward(got, dz, up, *out[2:], gamma, rms, dtype, rtype or dtype, (dtype, cols, rms))
+        a, b = dz.clone(), up.clone() if rtype else None
+        dg, db = torch.empty_like(gamma), None if rms else torch.empty_like(gamma)
+        hk.add_ln_q8_bwd(a, b, *out[2:], gamma, a, b, dg, db, rms)
+        assert torch.equal(a, got[0]) and (b is None or torch.equal(b, got[1])) and torch.equal(dg, got[2])
+        assert rms or torch.equal(db, got[3])
+        dx = torch.empty_like(dz)
+        hk.add_ln_q8_bwd(dz, up, *out[2:], gamma, dx, None, None, None, rms)      # without the sums
+        assert torch.equal(dx, got[0])
+
+
 @pytest.mark.parametrize("rows,cols", [(5000, 96), (3001, 1021), (2600, 4096), (9000, 64), (40000, 8)])
 def test_many_rows(hk, cuda, rows, cols):
     """More rows than workgroups: the backward's workgroups walk."""
