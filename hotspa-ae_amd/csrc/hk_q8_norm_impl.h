@@ -503,6 +503,7 @@ static int launch_q8_norm_few_shape(const Q8BwdArgs& a, bool is_rms, const Q8Sha
     case 4: HK_Q8_FEW(4); break;
     default:
       if constexpr (q8_vec<T, RT>() == 4) HK_Q8_FEW(8);
+      else HK_REQUIRE(false, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
       break;
   }
 #undef HK_Q8_FEW
@@ -627,13 +628,18 @@ static int launch_q8_norm(const A& a, bool is_rms, const Q8Shape& shape, hipStre
       break;
     default:
       switch (shape.nv) {
-        case 1: HK_Q8(1, 0); break;
+        case 1:   // (where the shapes' rules give one)
+          if constexpr (WHAT == 1 && q8_vec<T, RT>() == 8) HK_Q8(1, 0);
+          else HK_REQUIRE(false, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
+          break;
         case 2: HK_Q8(2, 0); break;
         case 4:   // (the backward of wider rows takes another way)
           if constexpr (WHAT == 0 || q8_vec<T, RT>() == 4) HK_Q8(4, 0);
+          else HK_REQUIRE(false, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
           break;
         default:
           if constexpr (WHAT == 0 && q8_vec<T, RT>() == 4) HK_Q8(8, 0);
+          else HK_REQUIRE(false, HK_ERR_UNSUPPORTED, "q8_norm: no kernel for %d vectors a thread", shape.nv);
           break;
       }
   }
