@@ -538,7 +538,7 @@ void token_logprob_combine_kernel(LogprobCombineArgs a) {
       const uint32_t k = i < total ? lk[i] : 0;
       const int64_t tok = i < total ? lt[i] : 0;
       const uint64_t mask = __builtin_amdgcn_ballot_w64(k >= bound);
-      __syncthreads();   // (a place that is written was read in this round or before it)
+      __syncthreads();   // (a place that is written was read in this step or before it)
       if (k >= bound) {
         const int to = left + __builtin_popcountll(mask & ((uint64_t(1) << lane) - 1));
         lk[to] = k;
